@@ -502,6 +502,108 @@ LVB_API int lvb_embedding(const int64_t *ids, int64_t tokens, const uint16_t *ta
                           int64_t vocab_end, int64_t hidden_size, uint16_t *out, int64_t out_stride,
                           lvb_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* 8-bit paged K/V cache                                                     */
+/* ------------------------------------------------------------------------ */
+/* One layer holds, for the keys and for the values, codes [num_blocks]
+ * [num_kv_heads][block_size][head_size] of one byte (int8, or e4m3 floating
+ * point) and scales fp32 [num_blocks][num_kv_heads]; a code c of a block and
+ * head stands for c * scale.  Per-step metadata (block tables, computed
+ * counts, query starts) is that of the 16-bit cache above, and so is the
+ * place of a token: block table[p / block_size], slot p % block_size.
+ * Head sizes 64 and 128, block sizes that are multiples of 16 up to 1024
+ * (LVB_ERR_UNSUPPORTED for others).  What only the device can see -- query
+ * starts outside the batch, a request longer than max_query_len or than its
+ * table, block ids and positions out of range -- sets LVB_DEVERR_INDEX and
+ * the request, block or row concerned is left out.  The light-vllm
+ * repository has no 8-bit cache; the 16-bit counterparts are
+ * runtime/execution/paged_cache.py:30-338 and triton_paged_attention.py. */
+enum lvb_kv8_code { LVB_KV8_INT8 = 0, LVB_KV8_E4M3 = 1 };
+
+/* Append this step's K/V rows, and rotate its queries and keys on the way.
+ * positions (int32, one per token) with cos / sin [table_rows][head_size] of
+ * the rows' dtype: keys are rotated (half rotation, as lvb_rope_qk) in fp32
+ * and quantised without a rounding between, and `query` rows, if given, are
+ * rotated into `query_out` (may be `query` itself).  positions == NULL:
+ * nothing is rotated, query must be NULL.  Heads contiguous at stride
+ * head_size, token strides in elements.  For every block that receives
+ * tokens, per KV head and separately for keys and values: the scale becomes
+ * the larger of its present value (if the block holds tokens of earlier
+ * steps) and the new tokens' largest magnitude / M (M = 127 for int8, 448
+ * for e4m3), earlier tokens' codes are rounded anew if the scale grew, and
+ * the new tokens' codes are round(x / scale).  Slots past the request's end
+ * are left as they are.  A block must not be shared by requests that write
+ * to it (the rule of lvb_pack_step_metadata). */
+LVB_API int lvb_kv8_append(const uint16_t *query, int64_t query_token_stride, uint16_t *query_out,
+                           int64_t query_out_stride, const uint16_t *key, int64_t key_token_stride,
+                           const uint16_t *value, int64_t value_token_stride, const int32_t *positions,
+                           const uint16_t *cos_table, const uint16_t *sin_table, int64_t table_rows, void *key_codes,
+                           void *value_codes, float *key_scales, float *value_scales, const int32_t *block_tables,
+                           int64_t table_stride, const int32_t *num_computed, const int32_t *query_start_loc,
+                           int64_t num_seqs, int64_t num_tokens, int64_t max_query_len, int64_t num_query_heads,
+                           int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks, int dtype,
+                           int code_type, lvb_stream_t stream);
+
+/* Values of whole blocks: key_out / value_out [num_ids][num_kv_heads]
+ * [block_size][head_size] of `dtype`, code * scale rounded once; zeros for a
+ * block id out of range (which sets LVB_DEVERR_INDEX). */
+LVB_API int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, const float *key_scales,
+                                const float *value_scales, const int32_t *block_ids, int64_t num_ids,
+                                uint16_t *key_out, uint16_t *value_out, int64_t num_kv_heads, int64_t head_size,
+                                int64_t block_size, int64_t num_blocks, int dtype, int code_type,
+                                lvb_stream_t stream);
+
+/* out[t][h] = softmax(scale * q[t][h] . K^T) V over the positions up to and
+ * including token t's own (linear layouts: single tokens, drafted tokens
+ * under verification, prompt chunks, any mix), K and V read from the 8-bit
+ * cache, which must hold this step's tokens already (lvb_kv8_append).
+ * Softmax statistics and sums in fp32.  max_query_len is the longest request
+ * of the batch (LVB_DEVERR_INDEX and no output for a longer one); max_seq_len
+ * guides how contexts are split and need not be exact.  workspace: the bytes
+ * that lvb_kv8_attention_workspace_bytes gives for the same arguments (0:
+ * none), 16-byte aligned, zero-filled once; every call leaves it as it needs
+ * it.  Calls sharing a workspace must not overlap on the GPU. */
+LVB_API size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
+                                                 int64_t head_size, int64_t max_query_len, int64_t max_seq_len);
+LVB_API int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
+                              const void *value_codes, const float *key_scales, const float *value_scales,
+                              uint16_t *out, int64_t out_token_stride, const int32_t *block_tables,
+                              int64_t table_stride, const int32_t *num_computed, const int32_t *query_start_loc,
+                              int64_t num_seqs, int64_t num_tokens, int64_t max_query_len, int64_t max_seq_len,
+                              int64_t num_query_heads, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
+                              int64_t num_blocks, float scale, int dtype, int code_type, void *workspace,
+                              size_t workspace_bytes, lvb_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Verification of drafted tokens                                            */
+/* ------------------------------------------------------------------------ */
+/* Speculative sampling over a verification step's packed requests: request b
+ * owns the rows query_start_loc[b] .. [b + 1] of target_probs (fp32
+ * [num_rows][vocab_size], row stride in elements), one more than its drafts;
+ * drafts, their uniform numbers and their rows of draft_probs are packed
+ * without the extra row (request b's first at query_start_loc[b] - b).
+ * Draft x_i is accepted while accept_uniform * q_i(x_i) < p_i(x_i) (q_i = 1
+ * where draft_probs is NULL: drafts that were looked up, not drawn); after
+ * the accepted ones one token is drawn, by inverting the distribution
+ * function at sample_uniform[b] in whole numbers of 2^-40, from max(p - q, 0)
+ * at a refused draft (q one-hot where draft_probs is NULL; p itself if that
+ * is zero everywhere) or from the last row.  out_tokens [num_seqs]
+ * [max_query_len]: the accepted drafts, the drawn token, -1 for the rest;
+ * num_accepted: drafts accepted.  A request without rows, with rows outside
+ * the batch or with more than max_query_len sets LVB_DEVERR_INDEX and gets -1
+ * throughout and 0 accepted.  A drafted token outside the vocabulary is refused and sets
+ * LVB_DEVERR_INDEX.  Weights that are NaN or negative count as 0.
+ * workspace: lvb_verify_drafts_workspace_bytes() bytes (0: none), 16-byte
+ * aligned, zero-filled once; calls sharing one must not overlap on the GPU.
+ * The reference accepts drafts by greedy comparison only
+ * (runtime/execution/speculative.py). */
+LVB_API size_t lvb_verify_drafts_workspace_bytes(int64_t num_seqs, int64_t vocab_size);
+LVB_API int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const float *draft_probs,
+                              int64_t draft_stride, const int64_t *draft_tokens, const float *accept_uniform,
+                              const float *sample_uniform, const int32_t *query_start_loc, int64_t *out_tokens,
+                              int32_t *num_accepted, int64_t num_seqs, int64_t num_rows, int64_t max_query_len,
+                              int64_t vocab_size, void *workspace, size_t workspace_bytes, lvb_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -10,23 +10,36 @@ Two drop-in plugins behind light-vllm's own extension points:
 plus ``TensorParallelCollectives`` for the row-parallel all-reduce on the
 caller's stream (``light_vllm_b200.collectives``) and ``compact_kv``, the
 tree-acceptance K/V compaction on the device (``light_vllm_b200.kv_cache``).
-Both plugins take light-vllm's own ``PagedKVCache`` and
+A third part serves speculative decoding over a cache held in 8 bits:
+``kv8_append`` / ``kv8_attention`` / ``kv8_read_blocks`` over ``KV8Layer`` and
+``KV8Step`` (``light_vllm_b200.kv8``), and ``verify_drafts``
+(``light_vllm_b200.speculative``).
+
+The plugins take light-vllm's own ``PagedKVCache`` and
 ``PagedAttentionMetadata`` objects; this package defines no copies of them.  All GPU work goes through
 the C-ABI library ``_lib/liblvb200.so`` (``include/lvb200.h``); there is no
 CPU or Triton fallback.
 """
 
 from light_vllm_b200.awq import B200AWQOperation, B200AWQScheme, b200_awq_dequantize, b200_awq_linear
+from light_vllm_b200.kv8 import KV8Layer, KV8Step, kv8_append, kv8_attention, kv8_read_blocks
 from light_vllm_b200.kv_cache import KVCacheError, compact_kv
 from light_vllm_b200.paged_attention import B200PagedAttention, B200PagedAttentionBackend
+from light_vllm_b200.speculative import verify_drafts
 
 __all__ = [
     "B200AWQOperation",
     "B200AWQScheme",
     "B200PagedAttention",
     "B200PagedAttentionBackend",
+    "KV8Layer",
+    "KV8Step",
     "KVCacheError",
     "b200_awq_dequantize",
     "b200_awq_linear",
     "compact_kv",
+    "kv8_append",
+    "kv8_attention",
+    "kv8_read_blocks",
+    "verify_drafts",
 ]

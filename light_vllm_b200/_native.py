@@ -19,7 +19,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblvb200.so"
 HOSTPACK_PATH = Path(__file__).resolve().parent / "_lib" / ("_hostpack" + sysconfig.get_config_var("EXT_SUFFIX"))
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 LVB_OK = 0
 LVB_ERR_INVALID = 1
@@ -30,6 +30,9 @@ LVB_ERR_METADATA = 5
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
+
+KV8_INT8 = 0
+KV8_E4M3 = 1
 
 _c_ptr = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -132,6 +135,27 @@ PROTOTYPES: dict[str, tuple[object, tuple[object, ...]]] = {
         (_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr,
          _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int,
          _c_ptr, _size, _c_ptr),
+    ),
+    "lvb_kv8_append": (
+        _int,
+        (_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr,
+         _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _c_ptr),
+    ),
+    "lvb_kv8_read_blocks": (
+        _int,
+        (_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _int, _int, _c_ptr),
+    ),
+    "lvb_kv8_attention_workspace_bytes": (_size, (_i64, _i64, _i64, _i64, _i64, _i64)),
+    "lvb_kv8_attention": (
+        _int,
+        (_c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _c_ptr, _size, _c_ptr),
+    ),
+    "lvb_verify_drafts_workspace_bytes": (_size, (_i64, _i64)),
+    "lvb_verify_drafts": (
+        _int,
+        (_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _c_ptr,
+         _size, _c_ptr),
     ),
 }
 

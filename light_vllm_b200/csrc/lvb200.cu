@@ -15,6 +15,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -26,13 +27,16 @@
 #include "awq_decode.cuh"
 #include "awq_i8.cuh"
 #include "allreduce.cuh"
+#include "kv8_attention.cuh"
+#include "kv8_cache.cuh"
 #include "lvb_common.cuh"
 #include "paged_attention.cuh"
+#include "spec_verify.cuh"
 #include "step_metadata.cuh"
 
 namespace {
 
-constexpr int kAbiVersion = 8;
+constexpr int kAbiVersion = 9;
 constexpr int kMaxDevices = 64;
 
 thread_local char g_last_error[512] = "";
@@ -2075,4 +2079,233 @@ int lvb_silu_mul(const uint16_t *gate_up, int64_t in_stride, int64_t tokens, int
   cudaError_t e = launch_pdl(lvb::q2::silu_mul_kernel, dim3(static_cast<unsigned>(blocks)),
                              dim3(lvb::q2::kSiluThreads), 0, reinterpret_cast<cudaStream_t>(stream), a);
   return e == cudaSuccess ? LVB_OK : cuda_fail(e, "silu_mul_kernel launch");
+}
+
+// ------------------------------------------------------------------------
+// 8-bit paged cache and draft verification
+// ------------------------------------------------------------------------
+namespace {
+
+// Checks shared by the entry points over the 8-bit cache; fills `s`.
+int kv8_step(const char *what, lvb::kv8::Step &s, const int32_t *tables, int64_t table_stride, const int32_t *computed,
+             const int32_t *qsl, int64_t num_seqs, int64_t num_tokens, int64_t max_query_len, int64_t hkv, int64_t d,
+             int64_t bs, int64_t num_blocks, int dtype, int code) {
+  if (dtype != LVB_DTYPE_F16 && dtype != LVB_DTYPE_BF16) return fail(LVB_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  if (code != LVB_KV8_INT8 && code != LVB_KV8_E4M3) return fail(LVB_ERR_INVALID, "%s: unknown code type %d", what, code);
+  if (num_seqs < 0 || num_seqs > 65535 || num_tokens < 0 || num_tokens > INT_MAX || max_query_len < 0 ||
+      max_query_len > INT_MAX || table_stride < 0 || table_stride > INT_MAX || num_blocks <= 0 || num_blocks > INT_MAX)
+    return fail(LVB_ERR_INVALID, "%s: invalid batch size", what);
+  if (hkv <= 0 || hkv > 65535) return fail(LVB_ERR_INVALID, "%s: invalid KV head count %lld", what, (long long)hkv);
+  if (d != 64 && d != 128)
+    return fail(LVB_ERR_UNSUPPORTED, "%s: head size %lld (64 and 128 are covered)", what, (long long)d);
+  if (bs <= 0 || bs % 16 || bs > 1024)
+    return fail(LVB_ERR_UNSUPPORTED, "%s: block size %lld (multiples of 16 up to 1024 are covered)", what, (long long)bs);
+  if (num_seqs > 0 && (!tables || !computed || !qsl)) return fail(LVB_ERR_INVALID, "%s: null pointer argument", what);
+  s.tables = tables;
+  s.table_stride = table_stride;
+  s.computed = computed;
+  s.qsl = qsl;
+  s.num_seqs = static_cast<int>(num_seqs);
+  s.num_tokens = static_cast<int>(num_tokens);
+  s.max_query_len = static_cast<int>(max_query_len);
+  s.num_blocks = static_cast<int>(num_blocks);
+  s.bs = static_cast<int>(bs);
+  s.hkv = static_cast<int>(hkv);
+  return LVB_OK;
+}
+
+int kv8_layer_pointers(const char *what, const void *kc, const void *vc, const float *ks, const float *vs) {
+  if (!kc || !vc || !ks || !vs) return fail(LVB_ERR_INVALID, "%s: null pointer argument", what);
+  if (!aligned16(kc) || !aligned16(vc)) return fail(LVB_ERR_INVALID, "%s: codes must be 16-byte aligned", what);
+  return LVB_OK;
+}
+
+// Run `f` with the compile-time (bf16, e4m3, head size) of a call.
+template <typename F>
+cudaError_t kv8_dispatch(int dtype, int code, int64_t d, F &&f) {
+  using std::false_type;
+  using std::true_type;
+  auto by_d = [&](auto b16, auto fp8) {
+    return d == 128 ? f(b16, fp8, std::integral_constant<int, 128>{}) : f(b16, fp8, std::integral_constant<int, 64>{});
+  };
+  auto by_code = [&](auto b16) { return code == LVB_KV8_E4M3 ? by_d(b16, true_type{}) : by_d(b16, false_type{}); };
+  return dtype == LVB_DTYPE_BF16 ? by_code(true_type{}) : by_code(false_type{});
+}
+
+}  // namespace
+
+int lvb_kv8_append(const uint16_t *query, int64_t query_token_stride, uint16_t *query_out, int64_t query_out_stride,
+                   const uint16_t *key, int64_t key_token_stride, const uint16_t *value, int64_t value_token_stride,
+                   const int32_t *positions, const uint16_t *cos_table, const uint16_t *sin_table, int64_t table_rows,
+                   void *key_codes, void *value_codes, float *key_scales, float *value_scales,
+                   const int32_t *block_tables, int64_t table_stride, const int32_t *num_computed,
+                   const int32_t *query_start_loc, int64_t num_seqs, int64_t num_tokens, int64_t max_query_len,
+                   int64_t num_query_heads, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
+                   int64_t num_blocks, int dtype, int code_type, lvb_stream_t stream) {
+  lvb::kv8::AppendArgs a{};
+  int rc = kv8_step("kv8_append", a.step, block_tables, table_stride, num_computed, query_start_loc, num_seqs,
+                    num_tokens, max_query_len, num_kv_heads, head_size, block_size, num_blocks, dtype, code_type);
+  if (rc != LVB_OK) return rc;
+  if (num_query_heads < 0 || num_query_heads > 65535 || num_query_heads * num_tokens > INT_MAX)
+    return fail(LVB_ERR_INVALID, "kv8_append: invalid query head count %lld", (long long)num_query_heads);
+  if (num_seqs == 0 || num_tokens == 0) return LVB_OK;
+  rc = kv8_layer_pointers("kv8_append", key_codes, value_codes, key_scales, value_scales);
+  if (rc != LVB_OK) return rc;
+  if (!key || !value || (positions && (!cos_table || !sin_table)) || (query && (!query_out || !positions)))
+    return fail(LVB_ERR_INVALID, "kv8_append: null pointer argument");
+  if (key_token_stride < num_kv_heads * head_size || value_token_stride < num_kv_heads * head_size ||
+      (query && (query_token_stride < num_query_heads * head_size || query_out_stride < num_query_heads * head_size)))
+    return fail(LVB_ERR_INVALID, "kv8_append: token strides must cover the heads");
+  if (positions && (table_rows <= 0 || table_rows > INT_MAX))
+    return fail(LVB_ERR_INVALID, "kv8_append: invalid rotation table size %lld", (long long)table_rows);
+  a.query = query;
+  a.query_stride = query_token_stride;
+  a.query_out = query_out;
+  a.query_out_stride = query_out_stride;
+  a.key = key;
+  a.key_stride = key_token_stride;
+  a.value = value;
+  a.value_stride = value_token_stride;
+  a.positions = positions;
+  a.cos = cos_table;
+  a.sin = sin_table;
+  a.table_rows = static_cast<int>(table_rows);
+  a.hq = static_cast<int>(num_query_heads);
+  a.key_codes = static_cast<uint8_t *>(key_codes);
+  a.value_codes = static_cast<uint8_t *>(value_codes);
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.units = static_cast<int>(lvb::kv8::append_units(num_seqs, num_tokens, max_query_len, block_size));
+  constexpr int kWarps = lvb::kv8::kAppendThreads / 32;
+  const int64_t query_ctas = query != nullptr ? (num_query_heads * num_tokens + kWarps - 1) / kWarps : 0;
+  const dim3 grid(static_cast<unsigned>(a.units + std::min<int64_t>(query_ctas, 1 << 20)));
+  cudaError_t e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
+    return launch_pdl(lvb::kv8::append_kernel<decltype(b16)::value, decltype(fp8)::value, decltype(d)::value>, grid,
+                      dim3(lvb::kv8::kAppendThreads), 0, reinterpret_cast<cudaStream_t>(stream), a);
+  });
+  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 append_kernel launch");
+}
+
+int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, const float *key_scales,
+                        const float *value_scales, const int32_t *block_ids, int64_t num_ids, uint16_t *key_out,
+                        uint16_t *value_out, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
+                        int64_t num_blocks, int dtype, int code_type, lvb_stream_t stream) {
+  lvb::kv8::Step s{};
+  int rc = kv8_step("kv8_read_blocks", s, nullptr, 0, nullptr, nullptr, 0, 0, 0, num_kv_heads, head_size, block_size,
+                    num_blocks, dtype, code_type);
+  if (rc != LVB_OK) return rc;
+  if (num_ids < 0 || num_ids > INT_MAX) return fail(LVB_ERR_INVALID, "kv8_read_blocks: invalid block count");
+  if (num_ids == 0) return LVB_OK;
+  rc = kv8_layer_pointers("kv8_read_blocks", key_codes, value_codes, key_scales, value_scales);
+  if (rc != LVB_OK) return rc;
+  if (!block_ids || !key_out || !value_out) return fail(LVB_ERR_INVALID, "kv8_read_blocks: null pointer argument");
+  if (!aligned16(key_out) || !aligned16(value_out))
+    return fail(LVB_ERR_INVALID, "kv8_read_blocks: outputs must be 16-byte aligned");
+  lvb::kv8::ReadArgs a{};
+  a.key_codes = static_cast<const uint8_t *>(key_codes);
+  a.value_codes = static_cast<const uint8_t *>(value_codes);
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.ids = block_ids;
+  a.key_out = key_out;
+  a.value_out = value_out;
+  a.hkv = s.hkv;
+  a.num_blocks = s.num_blocks;
+  a.chunks_per_head = static_cast<int>(block_size * head_size / 16);
+  a.per_side = num_ids * num_kv_heads * a.chunks_per_head;
+  const int64_t ctas = (a.per_side + 255) / 256;
+  if (ctas > INT_MAX) return fail(LVB_ERR_UNSUPPORTED, "kv8_read_blocks: too many blocks in one call");
+  cudaError_t e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto) {
+    return launch_pdl(lvb::kv8::read_blocks_kernel<decltype(b16)::value, decltype(fp8)::value>,
+                      dim3(static_cast<unsigned>(ctas), 2), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), a);
+  });
+  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 read_blocks_kernel launch");
+}
+
+size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
+                                         int64_t head_size, int64_t max_query_len, int64_t max_seq_len) {
+  (void)num_seqs, (void)num_query_heads, (void)num_kv_heads, (void)head_size, (void)max_query_len, (void)max_seq_len;
+  return 0;
+}
+
+int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
+                      const void *value_codes, const float *key_scales, const float *value_scales, uint16_t *out,
+                      int64_t out_token_stride, const int32_t *block_tables, int64_t table_stride,
+                      const int32_t *num_computed, const int32_t *query_start_loc, int64_t num_seqs,
+                      int64_t num_tokens, int64_t max_query_len, int64_t max_seq_len, int64_t num_query_heads,
+                      int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks, float scale,
+                      int dtype, int code_type, void *workspace, size_t workspace_bytes, lvb_stream_t stream) {
+  (void)workspace, (void)workspace_bytes;
+  lvb::kv8::AttnArgs a{};
+  int rc = kv8_step("kv8_attention", a.step, block_tables, table_stride, num_computed, query_start_loc, num_seqs,
+                    num_tokens, max_query_len, num_kv_heads, head_size, block_size, num_blocks, dtype, code_type);
+  if (rc != LVB_OK) return rc;
+  if (num_query_heads <= 0 || num_query_heads % num_kv_heads || num_query_heads > 65535)
+    return fail(LVB_ERR_INVALID, "kv8_attention: %lld query heads over %lld KV heads", (long long)num_query_heads,
+                (long long)num_kv_heads);
+  if (max_seq_len < 0) return fail(LVB_ERR_INVALID, "kv8_attention: invalid longest sequence");
+  if (num_seqs == 0 || num_tokens == 0 || max_query_len == 0) return LVB_OK;
+  rc = kv8_layer_pointers("kv8_attention", key_codes, value_codes, key_scales, value_scales);
+  if (rc != LVB_OK) return rc;
+  if (!query || !out) return fail(LVB_ERR_INVALID, "kv8_attention: null pointer argument");
+  if (query_token_stride < num_query_heads * head_size || out_token_stride < num_query_heads * head_size)
+    return fail(LVB_ERR_INVALID, "kv8_attention: token strides must cover the heads");
+  a.query = query;
+  a.query_stride = query_token_stride;
+  a.out = out;
+  a.out_stride = out_token_stride;
+  a.key_codes = static_cast<const uint8_t *>(key_codes);
+  a.value_codes = static_cast<const uint8_t *>(value_codes);
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.hq = static_cast<int>(num_query_heads);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const dim3 grid(static_cast<unsigned>(max_query_len), static_cast<unsigned>(num_query_heads),
+                  static_cast<unsigned>(num_seqs));
+  cudaError_t e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
+    return launch_pdl(lvb::kv8::attention_kernel<decltype(b16)::value, decltype(fp8)::value, decltype(d)::value>, grid,
+                      dim3(32), 0, reinterpret_cast<cudaStream_t>(stream), a);
+  });
+  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 attention_kernel launch");
+}
+
+size_t lvb_verify_drafts_workspace_bytes(int64_t num_seqs, int64_t vocab_size) {
+  (void)num_seqs, (void)vocab_size;
+  return 0;
+}
+
+int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const float *draft_probs, int64_t draft_stride,
+                      const int64_t *draft_tokens, const float *accept_uniform, const float *sample_uniform,
+                      const int32_t *query_start_loc, int64_t *out_tokens, int32_t *num_accepted, int64_t num_seqs,
+                      int64_t num_rows, int64_t max_query_len, int64_t vocab_size, void *workspace,
+                      size_t workspace_bytes, lvb_stream_t stream) {
+  (void)workspace, (void)workspace_bytes;
+  if (num_seqs < 0 || num_seqs > INT_MAX || num_rows < 0 || num_rows > INT_MAX || max_query_len < 0 ||
+      max_query_len > INT_MAX || vocab_size <= 0 || vocab_size > INT_MAX)
+    return fail(LVB_ERR_INVALID, "verify_drafts: invalid batch or vocabulary size");
+  if (num_seqs == 0) return LVB_OK;
+  if (num_rows < num_seqs) return fail(LVB_ERR_INVALID, "verify_drafts: every request needs a row");
+  if (target_stride < vocab_size || (draft_probs && draft_stride < vocab_size))
+    return fail(LVB_ERR_INVALID, "verify_drafts: row strides must cover the vocabulary");
+  if (!query_start_loc || !num_accepted || (max_query_len > 0 && !out_tokens) || !target_probs ||
+      !sample_uniform || (num_rows > num_seqs && (!draft_tokens || !accept_uniform)))
+    return fail(LVB_ERR_INVALID, "verify_drafts: null pointer argument");
+  lvb::spec::VerifyArgs a{};
+  a.target = target_probs;
+  a.target_stride = target_stride;
+  a.draft = draft_probs;
+  a.draft_stride = draft_stride;
+  a.tokens = draft_tokens;
+  a.accept = accept_uniform;
+  a.sample = sample_uniform;
+  a.qsl = query_start_loc;
+  a.out = out_tokens;
+  a.accepted = num_accepted;
+  a.num_seqs = static_cast<int>(num_seqs);
+  a.num_rows = static_cast<int>(num_rows);
+  a.width = static_cast<int>(max_query_len);
+  a.vocab = static_cast<int>(vocab_size);
+  cudaError_t e = launch_pdl(lvb::spec::verify_kernel, dim3(static_cast<unsigned>(num_seqs)),
+                             dim3(lvb::spec::kVerifyThreads), 0, reinterpret_cast<cudaStream_t>(stream), a);
+  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "verify_kernel launch");
 }

@@ -1,0 +1,292 @@
+"""A paged K/V cache held in 8 bits, and attention over it.
+
+Codes of one byte (``torch.int8`` or ``torch.float8_e4m3fn``) with one fp32
+scale for each block and KV head, for the keys and for the values: half the
+bytes of the 16-bit cache (runtime/execution/paged_cache.py:30-338, which has no
+8-bit form), so twice the context fits and a decode step reads half as much.
+
+* ``kv8_append`` -- rotate a step's queries and keys and append its keys and
+  values (``lvb_kv8_append``);
+* ``kv8_attention`` -- attention of the step's packed queries over the cache
+  (``lvb_kv8_attention``): single tokens, drafts under verification, prompt
+  chunks, any mix;
+* ``kv8_read_blocks`` -- values of whole blocks in the model's type
+  (``lvb_kv8_read_blocks``);
+* ``KV8Cache`` and ``B200KV8AttentionBackend`` -- the same behind the contract
+  of ``B200PagedAttentionBackend``, so that ``Qwen2AWQRunner`` and light-vllm's
+  step handler run over the 8-bit cache unchanged.
+
+All of it runs on the current stream, allocates through torch and does not
+synchronise.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from light_vllm_b200 import _native
+from light_vllm_b200.kv_cache import KVCacheError
+
+_ACT_DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
+_CODE_DTYPES = {torch.int8: _native.KV8_INT8, torch.float8_e4m3fn: _native.KV8_E4M3}
+
+
+class KV8Layer(NamedTuple):
+    """One layer's cache: codes [num_blocks, kv_heads, block_size, head_size]
+    and fp32 scales [num_blocks, kv_heads], all contiguous."""
+
+    keys: Tensor
+    values: Tensor
+    key_scales: Tensor
+    value_scales: Tensor
+
+
+class KV8Step(NamedTuple):
+    """A step's packed requests: int32 tensors on the device as
+    ``lvb_pack_step_metadata`` lays them out, and two host numbers.
+    ``max_query_len`` is the longest request's query count; ``max_seq_len``
+    (computed and query tokens) guides how contexts are split."""
+
+    block_tables: Tensor  # [requests, blocks]
+    num_computed: Tensor  # [requests], tokens cached by earlier steps
+    query_start: Tensor  # [requests + 1], prefix sums of query lengths
+    max_query_len: int
+    max_seq_len: int
+
+
+def _check_layer(layer: KV8Layer) -> int:
+    """The layer's code type; raises ``KVCacheError`` for a malformed layer."""
+
+    keys, values, key_scales, value_scales = layer
+    code = _CODE_DTYPES.get(keys.dtype)
+    if code is None or values.dtype != keys.dtype:
+        raise KVCacheError("KV8 codes must be int8 or float8_e4m3fn, keys and values alike")
+    shape = keys.shape
+    if len(shape) != 4 or values.shape != shape:
+        raise KVCacheError("KV8 codes must be [num_blocks, kv_heads, block_size, head_size]")
+    if (key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32
+            or key_scales.shape != shape[:2] or value_scales.shape != shape[:2]):
+        raise KVCacheError("KV8 scales must be float32 [num_blocks, kv_heads]")
+    if not (keys.is_contiguous() and values.is_contiguous() and key_scales.is_contiguous()
+            and value_scales.is_contiguous()):
+        raise KVCacheError("KV8 codes and scales must be contiguous")
+    device = keys.get_device()
+    if (device < 0 or values.get_device() != device or key_scales.get_device() != device
+            or value_scales.get_device() != device):
+        raise KVCacheError("KV8 codes and scales must share one CUDA device")
+    return code
+
+
+def _check_step(step: KV8Step, device: int) -> int:
+    """The number of requests; raises ``KVCacheError`` for a malformed step."""
+
+    tables, computed, start = step[:3]
+    n = computed.shape[0]
+    if (tables.dtype != torch.int32 or computed.dtype != torch.int32 or start.dtype != torch.int32
+            or len(tables.shape) != 2 or len(computed.shape) != 1 or tables.shape[0] != n or start.shape != (n + 1,)):
+        raise KVCacheError("KV8 step metadata must be int32 [n, blocks], [n] and [n + 1]")
+    if (tables.get_device() != device or computed.get_device() != device or start.get_device() != device):
+        raise KVCacheError("KV8 step metadata must be on the cache's device")
+    if not computed.is_contiguous() or not start.is_contiguous() or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise KVCacheError("KV8 step metadata must be contiguous")
+    return n
+
+
+def _check_rows(name: str, rows: Tensor, tokens: int, heads: int | None, head_size: int, dtype: torch.dtype,
+                device: int) -> None:
+    shape = rows.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_size or (heads is not None and shape[1] != heads):
+        raise KVCacheError(f"KV8 {name} rows must be [tokens, heads, head_size] of the cache's heads")
+    if rows.dtype != dtype or rows.get_device() != device:
+        raise KVCacheError(f"KV8 {name} rows must share one dtype (fp16 or bf16) and the cache's device")
+
+
+def _dense_heads(rows: Tensor) -> Tensor:
+    """Rows whose heads are dense and in order (a token's stride is free)."""
+
+    if rows.is_contiguous() or (rows.stride(2) == 1 and rows.stride(1) == rows.shape[2]
+                                and rows.stride(0) >= rows.shape[1] * rows.shape[2]):
+        return rows
+    return rows.contiguous()
+
+
+class _Workspaces:
+    """Zero-filled scratch for each (device, stream); a call leaves it as it
+    needs it, and calls on one stream follow one another.  A grown buffer keeps
+    its predecessors, which a captured graph may still name."""
+
+    def __init__(self) -> None:
+        self._current: dict[tuple[int, int], Tensor] = {}
+        self._kept: list[Tensor] = []
+
+    def get(self, device: torch.device, stream: int, need: int) -> tuple[int, int]:
+        if need == 0:
+            return 0, 0
+        key = (device.index, stream)
+        buf = self._current.get(key)
+        if buf is None or buf.numel() < need:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("run the operator once on this stream before capturing it: its workspace is not "
+                                   "allocated yet")
+            if buf is not None:
+                self._kept.append(buf)
+            buf = torch.zeros(max(1 << 20, 1 << (need - 1).bit_length()), dtype=torch.uint8, device=device)
+            self._current[key] = buf
+        return buf.data_ptr(), buf.numel()
+
+
+_workspaces = _Workspaces()
+
+
+def kv8_append(query: Tensor | None, key: Tensor, value: Tensor, layer: KV8Layer, step: KV8Step, *,
+               positions: Tensor | None = None, cos: Tensor | None = None, sin: Tensor | None = None,
+               query_out: Tensor | None = None) -> Tensor | None:
+    """Append the step's key and value rows [tokens, kv_heads, head_size] to
+    ``layer`` and return the rotated query rows [tokens, heads, head_size].
+
+    With ``positions`` (int32, one for each token) and the tables ``cos`` /
+    ``sin`` [rows, head_size] of the rows' dtype, queries and keys are rotated
+    as ``lvb_rope_qk`` does; the keys go into the cache without a rounding
+    between.  Without them keys are appended as they are, and ``query`` must be
+    None.  ``query_out`` (``query`` itself, if wanted) receives the rotated
+    queries instead of a new tensor."""
+
+    code = _check_layer(layer)
+    keys = layer.keys
+    num_blocks, hkv, block, d = keys.shape
+    device = keys.device
+    index = device.index
+    n = _check_step(step, index)
+    dtype = key.dtype
+    act = _ACT_DTYPES.get(dtype)
+    if act is None:
+        raise KVCacheError("KV8 rows must be fp16 or bf16")
+    tokens = key.shape[0]
+    _check_rows("key", key, tokens, hkv, d, dtype, index)
+    _check_rows("value", value, tokens, hkv, d, dtype, index)
+    key, value = _dense_heads(key), _dense_heads(value)
+    pos_ptr = cos_ptr = sin_ptr = table_rows = q_ptr = q_stride = out_ptr = out_stride = hq = 0
+    if positions is not None:
+        if cos is None or sin is None:
+            raise KVCacheError("KV8 rotation needs the cos and sin tables")
+        if (positions.dtype != torch.int32 or positions.shape != (tokens,) or positions.get_device() != index
+                or not positions.is_contiguous()):
+            raise KVCacheError("KV8 positions must be int32, one for each token, on the cache's device")
+        if (cos.shape != sin.shape or len(cos.shape) != 2 or cos.shape[1] != d or cos.dtype != dtype
+                or sin.dtype != dtype or cos.get_device() != index or sin.get_device() != index
+                or not cos.is_contiguous() or not sin.is_contiguous()):
+            raise KVCacheError("KV8 rotation tables must be [rows, head_size] of the rows' dtype and device")
+        pos_ptr, cos_ptr, sin_ptr, table_rows = positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    if query is not None:
+        if positions is None:
+            raise KVCacheError("KV8 queries are only rotated: pass positions, or no query")
+        _check_rows("query", query, tokens, None, d, dtype, index)
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=dtype, device=device)
+        else:
+            _check_rows("query output", query_out, tokens, query.shape[1], d, dtype, index)
+            if _dense_heads(query_out) is not query_out:
+                raise KVCacheError("KV8 query output rows must have dense heads")
+        query = _dense_heads(query)
+        hq = query.shape[1]
+        q_ptr, q_stride, out_ptr, out_stride = (query.data_ptr(), query.stride(0), query_out.data_ptr(),
+                                                query_out.stride(0))
+    if tokens and n:
+        with _on(index):
+            _native.check(_native.library().lvb_kv8_append(
+                q_ptr, q_stride, out_ptr, out_stride, key.data_ptr(), key.stride(0), value.data_ptr(),
+                value.stride(0), pos_ptr, cos_ptr, sin_ptr, table_rows, keys.data_ptr(), layer.values.data_ptr(),
+                layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), step.block_tables.data_ptr(),
+                step.block_tables.stride(0), step.num_computed.data_ptr(), step.query_start.data_ptr(), n, tokens,
+                step.max_query_len, hq, hkv, d, block, num_blocks, act, code, _native.stream_handle(device)),
+                "lvb_kv8_append")
+    return query_out
+
+
+def kv8_read_blocks(layer: KV8Layer, block_ids: Tensor, *, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    """Keys and values [n, kv_heads, block_size, head_size] of the blocks
+    ``block_ids`` (int32 on the cache's device) in ``dtype``."""
+
+    code = _check_layer(layer)
+    act = _ACT_DTYPES.get(dtype)
+    if act is None:
+        raise KVCacheError("KV8 blocks are read in fp16 or bf16")
+    keys = layer.keys
+    num_blocks, hkv, block, d = keys.shape
+    device = keys.device
+    if (block_ids.dtype != torch.int32 or len(block_ids.shape) != 1 or block_ids.get_device() != device.index
+            or not block_ids.is_contiguous()):
+        raise KVCacheError("KV8 block ids must be a contiguous int32 vector on the cache's device")
+    n = block_ids.shape[0]
+    out = torch.empty((2, n, hkv, block, d), dtype=dtype, device=device)
+    key_out, value_out = out[0], out[1]
+    if n:
+        with _on(device.index):
+            _native.check(_native.library().lvb_kv8_read_blocks(
+                keys.data_ptr(), layer.values.data_ptr(), layer.key_scales.data_ptr(), layer.value_scales.data_ptr(),
+                block_ids.data_ptr(), n, key_out.data_ptr(), value_out.data_ptr(), hkv, d, block, num_blocks, act,
+                code, _native.stream_handle(device)), "lvb_kv8_read_blocks")
+    return key_out, value_out
+
+
+def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float, out: Tensor | None = None) -> Tensor:
+    """Attention of the step's query rows [tokens, heads, head_size] over
+    ``layer``, which must hold the step's own tokens already: token t of a
+    request sees every position up to its own.  ``out`` receives the result
+    instead of a new tensor."""
+
+    code = _check_layer(layer)
+    keys = layer.keys
+    num_blocks, hkv, block, d = keys.shape
+    device = keys.device
+    index = device.index
+    n = _check_step(step, index)
+    dtype = query.dtype
+    act = _ACT_DTYPES.get(dtype)
+    if act is None:
+        raise KVCacheError("KV8 rows must be fp16 or bf16")
+    tokens = query.shape[0]
+    _check_rows("query", query, tokens, None, d, dtype, index)
+    hq = query.shape[1]
+    if hq == 0 or hq % hkv:
+        raise KVCacheError("KV8 query heads must be a multiple of the KV heads")
+    if out is None:
+        out = torch.empty(query.shape, dtype=dtype, device=device)
+    else:
+        _check_rows("output", out, tokens, hq, d, dtype, index)
+        if _dense_heads(out) is not out:
+            raise KVCacheError("KV8 output rows must have dense heads")
+    query = _dense_heads(query)
+    if tokens and n:
+        with _on(index):
+            lib = _native.library()
+            stream = _native.stream_handle(device)
+            need = lib.lvb_kv8_attention_workspace_bytes(n, hq, hkv, d, step.max_query_len, step.max_seq_len)
+            ws, ws_bytes = _workspaces.get(device, stream, need)
+            _native.check(lib.lvb_kv8_attention(
+                query.data_ptr(), query.stride(0), keys.data_ptr(), layer.values.data_ptr(),
+                layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), out.data_ptr(), out.stride(0),
+                step.block_tables.data_ptr(), step.block_tables.stride(0), step.num_computed.data_ptr(),
+                step.query_start.data_ptr(), n, tokens, step.max_query_len, step.max_seq_len, hq, hkv, d, block,
+                num_blocks, scale, act, code, ws, ws_bytes, stream), "lvb_kv8_attention")
+    return out
+
+
+class _Same:
+    def __enter__(self) -> None:
+        return None
+
+    def __exit__(self, *exc) -> None:
+        return None
+
+
+_SAME = _Same()
+
+
+def _on(index: int):
+    """The tensors' device made current (launches go to the current device)."""
+
+    return _SAME if torch.cuda.current_device() == index else torch.cuda.device(index)
