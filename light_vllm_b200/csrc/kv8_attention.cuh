@@ -4,22 +4,10 @@
 // code * key scale and v_j = code * value scale of j's block.
 #pragma once
 
-#include "kv8_cache.cuh"
+#include "kv8_decode.cuh"
 
 namespace lvb {
 namespace kv8 {
-
-struct AttnArgs {
-  Step step;
-  const uint16_t *query;
-  int64_t query_stride;
-  uint16_t *out;
-  int64_t out_stride;
-  const uint8_t *key_codes, *value_codes;
-  const float *key_scales, *value_scales;
-  int hq;
-  float scale_log2;  // softmax scale * log2(e)
-};
 
 // One warp for each (token, query head): lanes score 32 positions at a time,
 // an fp32 online softmax runs over them, and each lane owns D / 32 elements.
@@ -32,7 +20,9 @@ __global__ void __launch_bounds__(32) attention_kernel(const __grid_constant__ A
   const Step &s = a.step;
   const int lane = threadIdx.x, h = blockIdx.y, r = blockIdx.z;
   int q0, qlen, computed;
-  if (!request_range(s, r, q0, qlen, computed) || static_cast<int>(blockIdx.x) >= qlen) return;
+  if (!request_range(s, r, q0, qlen, computed) || static_cast<int>(blockIdx.x) >= qlen ||
+      qlen <= kMaxRows / a.group)
+    return;
   const int t = q0 + blockIdx.x;
   const int kvh = h / (a.hq / s.hkv);
   const int end = computed + blockIdx.x + 1;

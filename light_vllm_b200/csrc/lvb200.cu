@@ -2222,10 +2222,40 @@ int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, const fl
   return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 read_blocks_kernel launch");
 }
 
+namespace {
+
+// Workspace of an attention call: partial sums for two pieces of each CTA that
+// the decode kernel may run, then the item counters.  The counters' place is
+// the same for every call on a device, so that they stay zero whatever calls
+// share a buffer.
+struct Kv8Workspace {
+  size_t o, ml, counts;  // offsets
+};
+
+Kv8Workspace kv8_workspace(int sms) {
+  constexpr int kMaxCtasPerSm = 3;
+  const size_t slots = static_cast<size_t>(2) * kMaxCtasPerSm * sms * lvb::kv8::kMaxRows;
+  Kv8Workspace w{};
+  w.ml = w.o + slots * 128 * sizeof(float);
+  w.counts = round256(w.ml + slots * sizeof(float2));
+  return w;
+}
+
+template <bool kBf16, bool kFp8, int D, bool kRows8>
+cudaError_t launch_kv8_decode(const lvb::kv8::AttnArgs &a, int sms, cudaStream_t stream) {
+  using Cfg = lvb::kv8::DecodeCfg<kBf16, kFp8, D, kRows8>;
+  return launch_pdl(lvb::kv8::decode_kernel<kBf16, kFp8, D, kRows8>, dim3(static_cast<unsigned>(sms * Cfg::kCtasPerSm)),
+                    dim3(Cfg::kThreads), 0, stream, a);
+}
+
+}  // namespace
+
 size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
                                          int64_t head_size, int64_t max_query_len, int64_t max_seq_len) {
-  (void)num_seqs, (void)num_query_heads, (void)num_kv_heads, (void)head_size, (void)max_query_len, (void)max_seq_len;
-  return 0;
+  (void)num_query_heads, (void)head_size, (void)max_query_len, (void)max_seq_len;
+  int dev = 0;
+  if (num_seqs <= 0 || num_kv_heads <= 0 || current_device(&dev) != LVB_OK) return 0;
+  return round256(kv8_workspace(sm_count(dev)).counts + static_cast<size_t>(num_seqs) * num_kv_heads * 4);
 }
 
 int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
@@ -2235,7 +2265,6 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
                       int64_t num_tokens, int64_t max_query_len, int64_t max_seq_len, int64_t num_query_heads,
                       int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks, float scale,
                       int dtype, int code_type, void *workspace, size_t workspace_bytes, lvb_stream_t stream) {
-  (void)workspace, (void)workspace_bytes;
   lvb::kv8::AttnArgs a{};
   int rc = kv8_step("kv8_attention", a.step, block_tables, table_stride, num_computed, query_start_loc, num_seqs,
                     num_tokens, max_query_len, num_kv_heads, head_size, block_size, num_blocks, dtype, code_type);
@@ -2259,13 +2288,39 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
   a.key_scales = key_scales;
   a.value_scales = value_scales;
   a.hq = static_cast<int>(num_query_heads);
+  a.group = static_cast<int>(num_query_heads / num_kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid(static_cast<unsigned>(max_query_len), static_cast<unsigned>(num_query_heads),
-                  static_cast<unsigned>(num_seqs));
-  cudaError_t e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
-    return launch_pdl(lvb::kv8::attention_kernel<decltype(b16)::value, decltype(fp8)::value, decltype(d)::value>, grid,
-                      dim3(32), 0, reinterpret_cast<cudaStream_t>(stream), a);
-  });
+  int dev = 0;
+  rc = current_device(&dev);
+  if (rc != LVB_OK) return rc;
+  const int sms = sm_count(dev);
+  const Kv8Workspace w = kv8_workspace(sms);
+  const size_t need = w.counts + static_cast<size_t>(num_seqs) * num_kv_heads * 4;
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+    return fail(LVB_ERR_WORKSPACE, "kv8_attention: workspace of %zu bytes is below the %zu required", workspace_bytes, need);
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  a.part_o = reinterpret_cast<float *>(ws + w.o);
+  a.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
+  a.counts = reinterpret_cast<uint32_t *>(ws + w.counts);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t rows = max_query_len * a.group;
+  cudaError_t e = cudaSuccess;
+  if (a.group <= lvb::kv8::kMaxRows) {
+    e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
+      constexpr bool kB16 = decltype(b16)::value, kFp8 = decltype(fp8)::value;
+      return rows <= 8 ? launch_kv8_decode<kB16, kFp8, decltype(d)::value, true>(a, sms, st)
+                       : launch_kv8_decode<kB16, kFp8, decltype(d)::value, false>(a, sms, st);
+    });
+    if (e != cudaSuccess) return cuda_fail(e, "kv8 decode_kernel launch");
+  }
+  if (rows > lvb::kv8::kMaxRows) {
+    const dim3 grid(static_cast<unsigned>(max_query_len), static_cast<unsigned>(num_query_heads),
+                    static_cast<unsigned>(num_seqs));
+    e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
+      return launch_pdl(lvb::kv8::attention_kernel<decltype(b16)::value, decltype(fp8)::value, decltype(d)::value>, grid,
+                        dim3(32), 0, st, a);
+    });
+  }
   return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 attention_kernel launch");
 }
 

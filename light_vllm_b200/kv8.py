@@ -114,7 +114,7 @@ def _dense_heads(rows: Tensor) -> Tensor:
 
 
 class _Workspaces:
-    """Zero-filled scratch for each (device, stream); a call leaves it as it
+    """Zero-filled scratch of one operator for each (device, stream); a call leaves it as it
     needs it, and calls on one stream follow one another.  A grown buffer keeps
     its predecessors, which a captured graph may still name."""
 

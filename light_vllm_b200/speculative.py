@@ -15,7 +15,9 @@ import torch
 from torch import Tensor
 
 from light_vllm_b200 import _native
-from light_vllm_b200.kv8 import _on, _workspaces
+from light_vllm_b200.kv8 import _on, _Workspaces
+
+_workspaces = _Workspaces()
 
 
 def verify_drafts(target_probs: Tensor, draft_tokens: Tensor, accept_uniform: Tensor, sample_uniform: Tensor,
