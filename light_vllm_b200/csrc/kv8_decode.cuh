@@ -14,14 +14,15 @@
 // m and the scores are fp32.  m moves only when it would grow by more than kLazy:
 // a rescaling of O is rare.
 //
-// Tensor cores.  Both products are m16n8k16 warp MMAs with the query rows as M
-// (the tensor pipe is not what bounds this).  Codes are exact in fp16: int8 by
-// setting the byte under the exponent of 1024 and subtracting 1152, e4m3 by the
-// hardware's conversion.  Operands go from global memory straight to the
-// fragments' registers: the order of the head's elements in q k^T, and of a
-// page's 16 positions, is free as long as both operands agree, so lane (g, t) of
-// the fragment takes 16 consecutive bytes of key row g (its q fragments are laid
-// out alike) and 16 consecutive bytes of value rows 2t, 2t + 1, 2t + 8, 2t + 9.
+// Tensor cores.  Both products are m16n8k16 warp MMAs with 16 positions (then 16
+// elements of the head) as M and the query rows as N, so up to 8 rows waste
+// nothing.  Codes are exact in fp16: int8 by setting the byte under the exponent
+// of 1024 and subtracting 1152, e4m3 by the hardware's conversion.  The order of
+// the head's elements in q k^T, and of a page's positions, is free as long as
+// both operands agree, so lane (g, t) of the fragment takes 16 consecutive bytes
+// of key rows g and g + 8, and of value rows 2t, 2t + 1, 2t + 8, 2t + 9.  A lane
+// only ever reads what it fetched itself: asynchronous copies bring its pieces
+// of the next two pages into its own slots of shared memory, with no barrier.
 //
 // Split.  The pages of all (request, KV head) items are laid end to end and cut
 // into one equal run for each resident CTA, whatever the contexts' lengths; the
@@ -50,6 +51,7 @@ struct AttnArgs {
   const uint8_t *key_codes, *value_codes;
   const float *key_scales, *value_scales;
   int hq, group;
+  bool query_vec, out_vec;  // rows allow 16-byte loads, 8-byte stores
   float scale_log2;  // softmax scale * log2(e)
   // decode kernel
   float *part_o;      // [2 * CTAs][kMaxRows][D]
@@ -83,14 +85,6 @@ struct Pair<true> {
   }
 };
 
-// D += A B with rows 8..15 of A zero: half the accumulator registers.
-__device__ __forceinline__ void mma_rows8(float &d0, float &d1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  float x, y;
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%6,%5,%6}, {%7,%8}, {%0,%1,%9,%9};"
-      : "+f"(d0), "+f"(d1), "=f"(x), "=f"(y)
-      : "r"(a0), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
-}
-
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -101,6 +95,14 @@ __device__ __forceinline__ float log2_fast(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ void lds_16(uint32_t (&v)[4], uint32_t src) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+}
+
+__device__ __forceinline__ void lds_8(uint32_t (&v)[2], uint32_t src) {
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(src) : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) { return pack2<false>(lo, hi); }
@@ -131,32 +133,48 @@ struct Segment {
   int q0, rows, computed;
 };
 
-template <bool kBf16, bool kFp8, int D, bool kRows8>
+// kNT: tiles of 8 query rows.
+template <int D, int kNT>
 struct DecodeCfg {
-  static constexpr int kWarps = kRows8 ? 8 : 4;
+  static constexpr int kWarps = 8;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kCtasPerSm = kRows8 ? 2 : 3;
-  static constexpr int kRowSlots = kRows8 ? 8 : 16;
-  static constexpr int kPad = D + 4;  // a row of O in shared memory
+  static constexpr int kCtasPerSm = kNT == 1 ? 2 : 1;
+  static constexpr int kRows = 8 * kNT;
+  static constexpr int kPad = D + 4;                // floats of a row of O in shared memory
+  static constexpr int kPageBytes = 2 * kPage * D;  // K and V
+  static constexpr int kSlots = 2;                  // pages in flight for each warp
+  static constexpr int kRingBytes = kWarps * kSlots * kPageBytes;
+  static constexpr int kOBytes = kWarps * kRows * kPad * 4;
+  static constexpr int kSmemBytes = kRingBytes + kOBytes;
 };
 
-template <bool kBf16, bool kFp8, int D, bool kRows8>
-__global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, DecodeCfg<kBf16, kFp8, D, kRows8>::kCtasPerSm)
+__device__ __forceinline__ void cp_async_8(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool kBf16, bool kFp8, int D, int kNT>
+__global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>::kCtasPerSm)
     decode_kernel(const __grid_constant__ AttnArgs a) {
-  using Cfg = DecodeCfg<kBf16, kFp8, D, kRows8>;
+  using Cfg = DecodeCfg<D, kNT>;
   using P = Pair<kFp8>;
-  constexpr int kWarps = Cfg::kWarps, kThreads = Cfg::kThreads, kSlots = Cfg::kRowSlots;
-  constexpr int kKSteps = D / 16;   // MMAs of a score
-  constexpr int kNTiles = D / 8;    // MMAs of O
+  constexpr int kWarps = Cfg::kWarps, kThreads = Cfg::kThreads, kRows = Cfg::kRows;
+  constexpr int kKSteps = D / 16;   // MMAs of a score tile
+  constexpr int kDTiles = D / 16;   // MMAs of O
   constexpr int kKChunks = D / 64;  // 16-byte pieces of a key row that a lane takes
   constexpr int kVWords = D / 32;   // words of a value row that a lane takes
-  constexpr int kHalves = kRows8 ? 1 : 2;
-  __shared__ float o_sm[kWarps][kSlots][Cfg::kPad];
-  __shared__ float m_sm[kWarps][kSlots], l_sm[kWarps][kSlots];
+  constexpr float kNone = -1e30f;   // m before any position
+  extern __shared__ __align__(16) uint8_t smem[];
+  float *o_sm = reinterpret_cast<float *>(smem + Cfg::kRingBytes);  // [warp][row][kPad]
+  __shared__ float m_sm[kWarps][kRows], l_sm[kWarps][kRows];
   __shared__ int scan[kWarps];
-  __shared__ long long scan_total;
-  __shared__ int start_sm[2];  // first request of the run, its pages before the run
-  __shared__ int last_sm;
+  __shared__ long long start_pages;  // pages before the run's first request
+  __shared__ int start_request, last_sm;
   pdl_wait();
   const Step &s = a.step;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, D
   // Pages of request r's items (0: not this kernel's, or refused).
   auto request_pages = [&](int r) {
     int q0, n, c;
-    if (!request_range(s, r, q0, n, c) || n == 0 || n > kSlots / a.group) return 0;
+    if (!request_range(s, r, q0, n, c) || n == 0 || n > kRows / a.group) return 0;
     return (c + n + kPage - 1) / kPage;
   };
   // Exclusive prefix of a value over the CTA; `sum` is the total.
@@ -191,9 +209,10 @@ __global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, D
 
   // The whole batch's pages, the run of each CTA, and where this one's begins.
   long long total = 0;
+  int mine = 0, sum = 0, ex = 0;
   for (int base = 0; base < s.num_seqs; base += kThreads) {
-    int sum;
-    block_scan(base + tid < s.num_seqs ? request_pages(base + tid) : 0, sum);
+    mine = base + tid < s.num_seqs ? request_pages(base + tid) : 0;
+    ex = block_scan(mine, sum);
     total += static_cast<long long>(sum) * s.hkv;
   }
   long long run = (total + gridDim.x - 1) / gridDim.x;
@@ -204,21 +223,21 @@ __global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, D
   {
     long long before = 0;
     for (int base = 0; base < s.num_seqs; base += kThreads) {
-      const int mine = base + tid < s.num_seqs ? request_pages(base + tid) : 0;
-      int sum;
-      const int ex = block_scan(mine, sum);
+      if (s.num_seqs > kThreads) {
+        mine = base + tid < s.num_seqs ? request_pages(base + tid) : 0;
+        ex = block_scan(mine, sum);
+      }
       const long long lo = before + static_cast<long long>(ex) * s.hkv, hi = lo + static_cast<long long>(mine) * s.hkv;
       if (lo <= begin && begin < hi) {
-        start_sm[0] = base + tid;
-        scan_total = lo;
+        start_request = base + tid;
+        start_pages = lo;
       }
       before += static_cast<long long>(sum) * s.hkv;
     }
     __syncthreads();
   }
 
-  // Walk of the run: `at` is the flat index of segment `seg`'s first page.
-  auto describe = [&](int r, int kvh, int first, long long left, Segment &seg) {
+  auto describe = [&](int r, int kvh, int first, int left, Segment &seg) {
     seg.r = r;
     seg.kvh = kvh;
     seg.q0 = s.qsl[r];
@@ -227,65 +246,20 @@ __global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, D
     seg.rows = n * a.group;
     seg.pages = (seg.computed + n + kPage - 1) / kPage;
     seg.first = first;
-    seg.last = static_cast<int>(left < seg.pages - first ? first + left : seg.pages);
+    seg.last = left < seg.pages - first ? first + left : seg.pages;
   };
-  long long at = begin;
+  int left = static_cast<int>(end - begin);  // pages of the run from the present segment on
   Segment seg;
   {
-    const int r = start_sm[0];
+    const int r = start_request;
     const int pages = request_pages(r);
-    const int inside = static_cast<int>(begin - scan_total);
-    describe(r, inside / pages, inside % pages, end - begin, seg);
+    const int inside = static_cast<int>(begin - start_pages);
+    describe(r, inside / pages, inside % pages, left, seg);
   }
-
-  const int ppb = s.bs / kPage;
-  uint32_t kreg[2][kKChunks][4], vreg[4][kVWords];
-  float ks = 0.f, vs = 1.f;   // scales of the page in kreg / vreg
-  int bad = 0;                // its block id is out of range
-  int64_t head_at = 0;        // first byte of the next page's head
-  float ks_next, vs_next;
-  int bad_next;
-
-  // Start of page p of item (r, kvh): its place and scales.
-  auto locate = [&](int r, int kvh, int p) {
-    const int blk = ppb == 1 ? p : p / ppb;
-    int phys = s.tables[r * s.table_stride + blk];
-    bad_next = phys < 0 || phys >= s.num_blocks;
-    if (bad_next) {
-      record_device_error(LVB_DEVERR_INDEX);
-      phys = 0;
-    }
-    const int64_t h = static_cast<int64_t>(phys) * s.hkv + kvh;
-    ks_next = a.key_scales[h];
-    vs_next = a.value_scales[h];
-    head_at = (h * s.bs + (p - blk * ppb) * kPage) * D;
-  };
-  auto load_keys = [&]() {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < kKChunks; ++c) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(a.key_codes + head_at + (g + 8 * i) * D + c * 64 + t * 16));
-        kreg[i][c][0] = v.x, kreg[i][c][1] = v.y, kreg[i][c][2] = v.z, kreg[i][c][3] = v.w;
-      }
-  };
-  auto load_values = [&]() {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t *src = a.value_codes + head_at + (2 * t + (i & 1) + (i >> 1) * 8) * D + g * (D / 8);
-      if constexpr (D == 128) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src));
-        vreg[i][0] = v.x, vreg[i][1] = v.y, vreg[i][2] = v.z, vreg[i][3] = v.w;
-      } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
-        vreg[i][0] = v.x, vreg[i][1] = v.y;
-      }
-    }
-  };
-  // Item after (r, kvh); false at the end of the run.
+  // The segment after `from`; false at the end of the run.
   auto next_segment = [&](const Segment &from, Segment &to) {
-    const long long left = end - at - (from.last - from.first);
-    if (left <= 0) return false;
+    const int rest = left - (from.last - from.first);
+    if (rest <= 0) return false;
     int r = from.r, kvh = from.kvh + 1;
     if (kvh == s.hkv) {
       kvh = 0;
@@ -293,205 +267,294 @@ __global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, D
         ++r;
       } while (request_pages(r) == 0);  // pages are left, so a request is
     }
-    describe(r, kvh, 0, left, to);
+    describe(r, kvh, 0, rest, to);
     return true;
   };
 
-  bool more = true;
-  if (seg.first + warp < seg.last) {
-    locate(seg.r, seg.kvh, seg.first + warp);
-    load_keys();
-    load_values();
-  }
-  while (more) {
-    Segment nseg;
-    more = next_segment(seg, nseg);
-    // Query rows g and g + 8: row i is token i / group, head i % group.
-    uint32_t qa[kKSteps][kRows8 ? 2 : 4];
-    float f[kHalves];
-    int limit[kHalves];  // last position that the row sees
+  // This lane's pieces of a page: 2 kKChunks of 16 bytes of K, four of 4 kVWords bytes of V.
+  const uint32_t ring = smem_u32(smem) + warp * (Cfg::kSlots * Cfg::kPageBytes);
+  const int ppb = s.bs / kPage;
+  const uint32_t head_bytes = static_cast<uint32_t>(s.bs) * D;
+  const uint8_t *k_lane = a.key_codes + g * D + t * 16;
+  const uint8_t *v_lane = a.value_codes + 2 * t * D + g * (D / 8);
+  float ks_ring[Cfg::kSlots], vs_ring[Cfg::kSlots];  // scales; ks NaN: block id out of range
+  auto fetch = [&](const Segment &of, int p, int slot) {
+    const int blk = ppb == 1 ? p : p / ppb;
+    int phys = s.tables[of.r * s.table_stride + blk];
+    const bool bad = static_cast<uint32_t>(phys) >= static_cast<uint32_t>(s.num_blocks);
+    if (bad) {
+      record_device_error(LVB_DEVERR_INDEX);
+      phys = 0;
+    }
+    const uint32_t h = static_cast<uint32_t>(phys) * s.hkv + of.kvh;
+    ks_ring[slot] = bad ? NAN : __ldg(a.key_scales + h);
+    vs_ring[slot] = __ldg(a.value_scales + h);
+    const uint64_t at = static_cast<uint64_t>(h) * head_bytes + (p - blk * ppb) * (kPage * D);
+    const uint8_t *kp = k_lane + at, *vp = v_lane + at;
+    const uint32_t dst = ring + slot * Cfg::kPageBytes;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const int row = g + 8 * h;
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < kKChunks; ++c)
+        cp_async_16(dst + ((i * kKChunks + c) * 32 + lane) * 16, kp + i * 8 * D + c * 64, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t *src = vp + ((i & 1) + (i >> 1) * 8) * D;
+      if constexpr (D == 128)
+        cp_async_16(dst + kPage * D + (i * 32 + lane) * 16, src, 16);
+      else
+        cp_async_8(dst + kPage * D + (i * 32 + lane) * 8, src);
+    }
+  };
+
+  // Pages of the run that this warp takes, in order, across segments: (fs, fp)
+  // is the next one to fetch.
+  Segment fs = seg;
+  int fp = seg.first + warp;
+  int fleft = left;
+  bool fmore = true;
+  auto fetch_next = [&](int slot) {
+    while (fmore && fp >= fs.last) {
+      Segment n;
+      const int keep = left;
+      left = fleft;
+      fmore = next_segment(fs, n);
+      left = keep;
+      if (fmore) {
+        fleft -= fs.last - fs.first;
+        fs = n;
+        fp = fs.first + warp;
+      }
+    }
+    if (fmore) {
+      fetch(fs, fp, slot);
+      fp += kWarps;
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < Cfg::kSlots; ++i) fetch_next(i);
+  int slot = 0;
+
+  bool more = true;
+  while (more) {
+    // Query rows n = g (B fragments), and rows 2t, 2t + 1 (scores): row i is
+    // token i / group, head i % group.
+    uint32_t qb[kNT][kKSteps][2];
+    float f[kNT][2];
+    int limit[kNT][2];  // last position that the row sees
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      const int row = n * 8 + g;
       const bool ok = row < seg.rows;
       const int tok = ok ? row / a.group : 0, head = ok ? row - tok * a.group : 0;
       const uint16_t *src = a.query + (seg.q0 + tok) * a.query_stride + (seg.kvh * a.group + head) * D + t * 16;
       float x[kKChunks * 16];
 #pragma unroll
-      for (int c = 0; c < kKChunks; ++c)
+      for (int c = 0; c < kKChunks; ++c) {
+        if (a.query_vec) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[c * 16 + i] = ok ? to_float<kBf16>(src[c * 64 + i]) : 0.f;
+          for (int i = 0; i < 2; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (ok) v = *reinterpret_cast<const uint4 *>(src + c * 64 + i * 8);
+            const uint16_t *e = reinterpret_cast<const uint16_t *>(&v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[c * 16 + i * 8 + k] = to_float<kBf16>(e[k]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[c * 16 + i] = ok ? to_float<kBf16>(src[c * 64 + i]) : 0.f;
+        }
+      }
       const float up = query_shift<kBf16>(x);
-      f[h] = a.scale_log2 / up;
+      const float fr = a.scale_log2 / up;
+      const int lim = ok ? seg.computed + tok : -1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[n][e] = __shfl_sync(0xffffffffu, fr, (2 * t + e) * 4);
+        limit[n][e] = __shfl_sync(0xffffffffu, lim, (2 * t + e) * 4);
+      }
 #pragma unroll
       for (int k = 0; k < kKSteps; ++k) {
-        const int i = k * 4;
-        qa[k][h] = pack_half(x[i] * up, x[i + 1] * up);
-        qa[k][kHalves + h] = pack_half(x[i + 2] * up, x[i + 3] * up);
+        qb[n][k][0] = pack_half(x[4 * k] * up, x[4 * k + 1] * up);
+        qb[n][k][1] = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
       }
-      limit[h] = ok ? seg.computed + tok : -1;
     }
-    float o[kNTiles][2 * kHalves], m[kHalves], l[kHalves];
+    float o[kNT][kDTiles][4], m[kNT][2], l[kNT][2];
 #pragma unroll
-    for (int j = 0; j < kNTiles; ++j)
+    for (int n = 0; n < kNT; ++n) {
 #pragma unroll
-      for (int i = 0; i < 2 * kHalves; ++i) o[j][i] = 0.f;
+      for (int j = 0; j < kDTiles; ++j)
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) m[h] = -INFINITY, l[h] = 0.f;
+        for (int i = 0; i < 4; ++i) o[n][j][i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[n][e] = kNone, l[n][e] = 0.f;
+    }
 
-    const bool has_next_seg = more && nseg.first + warp < nseg.last;
     for (int p = seg.first + warp; p < seg.last; p += kWarps) {
-      ks = ks_next, vs = vs_next, bad = bad_next;
-      bool next = p + kWarps < seg.last;
-      if (next) {
-        locate(seg.r, seg.kvh, p + kWarps);
-      } else if (has_next_seg) {
-        locate(nseg.r, nseg.kvh, nseg.first + warp);
-        next = true;
+      cp_async_wait_group<Cfg::kSlots - 1>();
+      const uint32_t src = ring + slot * Cfg::kPageBytes;
+      const float ks = slot == 0 ? ks_ring[0] : ks_ring[1], vs = slot == 0 ? vs_ring[0] : vs_ring[1];
+      const bool bad = ks != ks;
+      uint32_t kreg[2][kKChunks][4], vreg[4][kVWords];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < kKChunks; ++c) lds_16(kreg[i][c], src + ((i * kKChunks + c) * 32 + lane) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (D == 128)
+          lds_16(vreg[i], src + kPage * D + (i * 32 + lane) * 16);
+        else
+          lds_8(vreg[i], src + kPage * D + (i * 32 + lane) * 8);
       }
-      // Scores of 16 positions: columns of two MMA tiles.
-      float sc[2][2 * kHalves];
+      // Scores: positions g and g + 8 by rows 2t and 2t + 1.
+      float sc[kNT][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int n = 0; n < kNT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2 * kHalves; ++e) sc[i][e] = 0.f;
+      for (int k = 0; k < kKSteps; ++k) {
+        const uint32_t w0 = P::bias(kreg[0][k >> 2][k & 3]), w1 = P::bias(kreg[1][k >> 2][k & 3]);
+        const uint32_t ka[4] = {P::template get<false>(w0), P::template get<false>(w1), P::template get<true>(w0),
+                                P::template get<true>(w1)};
 #pragma unroll
-        for (int k = 0; k < kKSteps; ++k) {
-          const uint32_t w = P::bias(kreg[i][k >> 2][k & 3]);
-          const uint32_t b0 = P::template get<false>(w), b1 = P::template get<true>(w);
-          if constexpr (kRows8)
-            mma_rows8(sc[i][0], sc[i][1], qa[k][0], qa[k][1], b0, b1);
-          else
-            mma_16816_nv<false>(sc[i], qa[k], b0, b1);
-        }
+        for (int n = 0; n < kNT; ++n) mma_16816_nv<false>(sc[n], ka, qb[n][k][0], qb[n][k][1]);
       }
-      if (next) load_keys();
       const float vw = vs > 0.f ? vs : 1.f;
-      const float lw = log2_fast(vw), iw = 1.f / vw;
-      const int pos = p * kPage + 2 * t;  // of column 0 of this lane
+      const float lw = log2_fast(vw), iw = rcp_fast(vw);
       const bool masked = bad || p * kPage + kPage - 1 > seg.computed;
-      float top[kHalves];
+      // Exponents against the present m, plus kHead.
+      float y[kNT][4];
+      auto exponents = [&]() {
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const float fk = f[h] * ks;
-        top[h] = -INFINITY;
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 4; ++i) y[n][i] = fmaf(sc[n][i], f[n][i & 1] * ks, lw - m[n][i & 1] + kHead);
+        if (masked) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = fmaf(sc[i][2 * h + e], fk, lw);
-            if (masked && (bad || pos + 8 * i + e > limit[h])) x = -INFINITY;
-            sc[i][2 * h + e] = x;
-            top[h] = fmaxf(top[h], x);
-          }
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      }
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (bad || p * kPage + g + (i >> 1) * 8 > limit[n][i & 1]) y[n][i] = -INFINITY;
+        }
+      };
+      exponents();
       bool grow = false;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) grow |= top[h] > m[h] + kLazy;
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) grow |= y[n][i] > kHead + kLazy;
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const float now = fmaxf(m[h], top[h]);
-          const float alpha = now == -INFINITY ? 1.f : exp2_fast(m[h] - now);
-          m[h] = now;
-          l[h] *= alpha;
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
-          for (int j = 0; j < kNTiles; ++j) o[j][2 * h] *= alpha, o[j][2 * h + 1] *= alpha;
-        }
+          for (int e = 0; e < 2; ++e) {
+            // the scores themselves: y is too coarse beside m = kNone
+            float top = m[n][e];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (y[n][2 * i + e] != -INFINITY) top = fmaxf(top, fmaf(sc[n][2 * i + e], f[n][e] * ks, lw));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float alpha = exp2_fast(m[n][e] - top);
+            m[n][e] = top;
+            l[n][e] *= alpha;
+#pragma unroll
+            for (int j = 0; j < kDTiles; ++j) o[n][j][e] *= alpha, o[n][j][2 + e] *= alpha;
+          }
+        exponents();
       }
-      uint32_t pa[2 * kHalves];
+      uint32_t pb[kNT][2];
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const float base = m[h] == -INFINITY ? 0.f : m[h] - kHead;
-        float e[2][2];
+      for (int n = 0; n < kNT; ++n) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          e[i][0] = exp2_fast(sc[i][2 * h] - base);
-          e[i][1] = exp2_fast(sc[i][2 * h + 1] - base);
-          pa[i * kHalves + h] = pack_half(e[i][0], e[i][1]);
-        }
-        l[h] = fmaf((e[0][0] + e[0][1]) + (e[1][0] + e[1][1]), iw, l[h]);
+        for (int i = 0; i < 4; ++i) y[n][i] = exp2_fast(y[n][i]);
+        l[n][0] = fmaf(y[n][0] + y[n][2], iw, l[n][0]);
+        l[n][1] = fmaf(y[n][1] + y[n][3], iw, l[n][1]);
+        pb[n][0] = movmatrix_trans(pack_half(y[n][0], y[n][1]));
+        pb[n][1] = movmatrix_trans(pack_half(y[n][2], y[n][3]));
       }
       if (kFp8 && masked) {
         // Slots past the end may hold NaN patterns: 0 * NaN is not 0.
+        const int stop = bad ? 0 : seg.computed + seg.rows / a.group;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (bad || p * kPage + 2 * t + (i & 1) + (i >> 1) * 8 >= seg.computed + seg.rows / a.group)
+          if (p * kPage + 2 * t + (i & 1) + (i >> 1) * 8 >= stop)
 #pragma unroll
             for (int w = 0; w < kVWords; ++w) vreg[i][w] = 0;
       }
+      // O: elements (D / 8) g + 2 j (rows g of the tile) and + 1 (rows g + 8).
 #pragma unroll
       for (int w = 0; w < kVWords; ++w) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          // bytes (2 half, 2 half + 1) of rows (0, 1) and (2, 3), interleaved
+          // bytes (2 half, 2 half + 1) of value rows (0, 1) and (2, 3), interleaved
           const uint32_t lo = P::bias(__byte_perm(vreg[0][w], vreg[1][w], half ? 0x7362 : 0x5140));
           const uint32_t hi = P::bias(__byte_perm(vreg[2][w], vreg[3][w], half ? 0x7362 : 0x5140));
-          const int j = w * 4 + half * 2;
-          if constexpr (kRows8) {
-            mma_rows8(o[j][0], o[j][1], pa[0], pa[1], P::template get<false>(lo), P::template get<false>(hi));
-            mma_rows8(o[j + 1][0], o[j + 1][1], pa[0], pa[1], P::template get<true>(lo), P::template get<true>(hi));
-          } else {
-            mma_16816_nv<false>(o[j], pa, P::template get<false>(lo), P::template get<false>(hi));
-            mma_16816_nv<false>(o[j + 1], pa, P::template get<true>(lo), P::template get<true>(hi));
-          }
+          const uint32_t va[4] = {P::template get<false>(lo), P::template get<true>(lo), P::template get<false>(hi),
+                                  P::template get<true>(hi)};
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) mma_16816_nv<false>(o[n][2 * w + half], va, pb[n][0], pb[n][1]);
         }
       }
-      if (next) load_values();
-    }
-    if (seg.first + warp >= seg.last && has_next_seg) {  // no page of this segment: fetch the next one's
-      locate(nseg.r, nseg.kvh, nseg.first + warp);
-      load_keys();
-      load_values();
+      // Everything of this slot is in registers and used: refill it.
+      if (slot == 0) fetch_next(0); else fetch_next(1);
+      slot ^= 1;
     }
 
-    // The warps' sums: O of row g at elements (D / 4) t + j and (D / 4) t + D / 8 + j.
+    // The warps' sums.
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int row = g + 8 * h;
-      if (t == 0) m_sm[warp][row] = m[h], l_sm[warp][row] = l[h];
+    for (int n = 0; n < kNT; ++n)
 #pragma unroll
-      for (int j = 0; j < kNTiles; ++j) {
-        o_sm[warp][row][t * (D / 4) + j] = o[j][2 * h];
-        o_sm[warp][row][t * (D / 4) + D / 8 + j] = o[j][2 * h + 1];
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        const int row = n * 8 + 2 * t + e;
+        if (g == 0) m_sm[warp][row] = m[n][e], l_sm[warp][row] = l[n][e];
+        float *dst = o_sm + (warp * kRows + row) * Cfg::kPad + g * (D / 8);
+#pragma unroll
+        for (int j = 0; j < kDTiles; j += 2)
+          *reinterpret_cast<float4 *>(dst + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
       }
-    }
     __syncthreads();
     const bool whole = seg.first == 0 && seg.last == seg.pages;
-    const int slot = 2 * blockIdx.x + (seg.first == 0 ? 1 : 0);
+    const int piece = 2 * blockIdx.x + (seg.first == 0 ? 1 : 0);
+    auto store = [&](int row, int d, float4 v, float total_l) {
+      const float inv = total_l > 0.f ? 1.f / total_l : 0.f;
+      const int tok = row / a.group, head = row - tok * a.group;
+      uint16_t *dst = a.out + (seg.q0 + tok) * a.out_stride + (seg.kvh * a.group + head) * D + d;
+      if (a.out_vec) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<kBf16>(v.x * inv, v.y * inv), pack2<kBf16>(v.z * inv, v.w * inv));
+      } else {
+        dst[0] = from_float<kBf16>(v.x * inv), dst[1] = from_float<kBf16>(v.y * inv);
+        dst[2] = from_float<kBf16>(v.z * inv), dst[3] = from_float<kBf16>(v.w * inv);
+      }
+    };
     for (int i = tid; i < seg.rows * (D / 4); i += kThreads) {
       const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-      float top = -INFINITY;
+      float top = kNone;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_sm[w][row]);
-      float sum = 0.f;
+      float sum_l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float wt = m_sm[w][row] == -INFINITY ? 0.f : exp2_fast(m_sm[w][row] - top);
-        const float4 v = *reinterpret_cast<const float4 *>(&o_sm[w][row][d]);
-        sum = fmaf(wt, l_sm[w][row], sum);
+        const float wt = exp2_fast(m_sm[w][row] - top);
+        const float4 v = *reinterpret_cast<const float4 *>(o_sm + (w * kRows + row) * Cfg::kPad + d);
+        sum_l = fmaf(wt, l_sm[w][row], sum_l);
         acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y);
         acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
       }
       if (whole) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        const int tok = row / a.group, head = row - tok * a.group;
-        uint16_t *dst = a.out + (seg.q0 + tok) * a.out_stride + (seg.kvh * a.group + head) * D + d;
-        dst[0] = from_float<kBf16>(acc.x * inv), dst[1] = from_float<kBf16>(acc.y * inv);
-        dst[2] = from_float<kBf16>(acc.z * inv), dst[3] = from_float<kBf16>(acc.w * inv);
+        store(row, d, acc, sum_l);
       } else {
-        *reinterpret_cast<float4 *>(a.part_o + (static_cast<int64_t>(slot) * kMaxRows + row) * D + d) = acc;
-        if (d == 0) a.part_ml[slot * kMaxRows + row] = make_float2(top, sum);
+        *reinterpret_cast<float4 *>(a.part_o + (static_cast<int64_t>(piece) * kMaxRows + row) * D + d) = acc;
+        if (d == 0) a.part_ml[piece * kMaxRows + row] = make_float2(top, sum_l);
       }
     }
     if (!whole) {
-      // The item's flat range, the CTAs that hold a piece of it, and how many.
-      const long long item = at - seg.first;
+      // The CTAs that hold a piece of the item.
+      const long long item = end - left - seg.first;
       const int c0 = static_cast<int>(item / run), c1 = static_cast<int>((item + seg.pages - 1) / run);
       uint32_t *count = a.counts + static_cast<int64_t>(seg.r) * s.hkv + seg.kvh;
       __threadfence();
@@ -503,33 +566,29 @@ __global__ void __launch_bounds__(DecodeCfg<kBf16, kFp8, D, kRows8>::kThreads, D
         if (tid == 0) *count = 0;
         for (int i = tid; i < seg.rows * (D / 4); i += kThreads) {
           const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-          float top = -INFINITY;
-          for (int c = c0; c <= c1; ++c) {
-            const int sl = 2 * c + (c == c0 ? 1 : 0);
-            top = fmaxf(top, __ldcg(&a.part_ml[sl * kMaxRows + row]).x);
-          }
-          float sum = 0.f;
+          float top = kNone;
+          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(&a.part_ml[(2 * c + (c == c0)) * kMaxRows + row]).x);
+          float sum_l = 0.f;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
           for (int c = c0; c <= c1; ++c) {
-            const int sl = 2 * c + (c == c0 ? 1 : 0);
-            const float2 ml = __ldcg(&a.part_ml[sl * kMaxRows + row]);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + (static_cast<int64_t>(sl) * kMaxRows + row) * D + d));
-            const float wt = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
-            sum = fmaf(wt, ml.y, sum);
+            const int at = (2 * c + (c == c0)) * kMaxRows + row;
+            const float2 ml = __ldcg(&a.part_ml[at]);
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + static_cast<int64_t>(at) * D + d));
+            const float wt = exp2_fast(ml.x - top);
+            sum_l = fmaf(wt, ml.y, sum_l);
             acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y);
             acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
           }
-          const float inv = sum > 0.f ? 1.f / sum : 0.f;
-          const int tok = row / a.group, head = row - tok * a.group;
-          uint16_t *dst = a.out + (seg.q0 + tok) * a.out_stride + (seg.kvh * a.group + head) * D + d;
-          dst[0] = from_float<kBf16>(acc.x * inv), dst[1] = from_float<kBf16>(acc.y * inv);
-          dst[2] = from_float<kBf16>(acc.z * inv), dst[3] = from_float<kBf16>(acc.w * inv);
+          store(row, d, acc, sum_l);
         }
       }
     }
     __syncthreads();  // o_sm is free again
-    at += seg.last - seg.first;
-    seg = nseg;
+    Segment n;
+    more = next_segment(seg, n);
+    left -= seg.last - seg.first;
+    if (more) seg = n;
   }
 }
 

@@ -2098,6 +2098,7 @@ int kv8_step(const char *what, lvb::kv8::Step &s, const int32_t *tables, int64_t
   if (hkv <= 0 || hkv > 65535) return fail(LVB_ERR_INVALID, "%s: invalid KV head count %lld", what, (long long)hkv);
   if (d != 64 && d != 128)
     return fail(LVB_ERR_UNSUPPORTED, "%s: head size %lld (64 and 128 are covered)", what, (long long)d);
+  if (num_blocks * hkv > INT_MAX) return fail(LVB_ERR_UNSUPPORTED, "%s: over 2^31 - 1 heads of blocks", what);
   if (bs <= 0 || bs % 16 || bs > 1024)
     return fail(LVB_ERR_UNSUPPORTED, "%s: block size %lld (multiples of 16 up to 1024 are covered)", what, (long long)bs);
   if (num_seqs > 0 && (!tables || !computed || !qsl)) return fail(LVB_ERR_INVALID, "%s: null pointer argument", what);
@@ -2122,7 +2123,7 @@ int kv8_layer_pointers(const char *what, const void *kc, const void *vc, const f
 
 // Run `f` with the compile-time (bf16, e4m3, head size) of a call.
 template <typename F>
-cudaError_t kv8_dispatch(int dtype, int code, int64_t d, F &&f) {
+auto kv8_dispatch(int dtype, int code, int64_t d, F &&f) {
   using std::false_type;
   using std::true_type;
   auto by_d = [&](auto b16, auto fp8) {
@@ -2233,7 +2234,7 @@ struct Kv8Workspace {
 };
 
 Kv8Workspace kv8_workspace(int sms) {
-  constexpr int kMaxCtasPerSm = 3;
+  constexpr int kMaxCtasPerSm = 2;
   const size_t slots = static_cast<size_t>(2) * kMaxCtasPerSm * sms * lvb::kv8::kMaxRows;
   Kv8Workspace w{};
   w.ml = w.o + slots * 128 * sizeof(float);
@@ -2241,11 +2242,16 @@ Kv8Workspace kv8_workspace(int sms) {
   return w;
 }
 
-template <bool kBf16, bool kFp8, int D, bool kRows8>
-cudaError_t launch_kv8_decode(const lvb::kv8::AttnArgs &a, int sms, cudaStream_t stream) {
-  using Cfg = lvb::kv8::DecodeCfg<kBf16, kFp8, D, kRows8>;
-  return launch_pdl(lvb::kv8::decode_kernel<kBf16, kFp8, D, kRows8>, dim3(static_cast<unsigned>(sms * Cfg::kCtasPerSm)),
-                    dim3(Cfg::kThreads), 0, stream, a);
+template <bool kBf16, bool kFp8, int D, int kNT>
+int launch_kv8_decode(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) {
+  using Cfg = lvb::kv8::DecodeCfg<D, kNT>;
+  static bool smem_done[kMaxDevices] = {false};
+  auto kernel = lvb::kv8::decode_kernel<kBf16, kFp8, D, kNT>;
+  int rc = ensure_smem(kernel, Cfg::kSmemBytes, dev, smem_done);
+  if (rc != LVB_OK) return rc;
+  cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(sm_count(dev) * Cfg::kCtasPerSm)), dim3(Cfg::kThreads),
+                             Cfg::kSmemBytes, stream, a);
+  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 decode_kernel launch");
 }
 
 }  // namespace
@@ -2289,6 +2295,8 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
   a.value_scales = value_scales;
   a.hq = static_cast<int>(num_query_heads);
   a.group = static_cast<int>(num_query_heads / num_kv_heads);
+  a.query_vec = aligned16(query) && query_token_stride % 8 == 0;
+  a.out_vec = (reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_token_stride % 4 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   int dev = 0;
   rc = current_device(&dev);
@@ -2306,12 +2314,12 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
   const int64_t rows = max_query_len * a.group;
   cudaError_t e = cudaSuccess;
   if (a.group <= lvb::kv8::kMaxRows) {
-    e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
+    rc = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
       constexpr bool kB16 = decltype(b16)::value, kFp8 = decltype(fp8)::value;
-      return rows <= 8 ? launch_kv8_decode<kB16, kFp8, decltype(d)::value, true>(a, sms, st)
-                       : launch_kv8_decode<kB16, kFp8, decltype(d)::value, false>(a, sms, st);
+      return rows <= 8 ? launch_kv8_decode<kB16, kFp8, decltype(d)::value, 1>(a, dev, st)
+                       : launch_kv8_decode<kB16, kFp8, decltype(d)::value, 2>(a, dev, st);
     });
-    if (e != cudaSuccess) return cuda_fail(e, "kv8 decode_kernel launch");
+    if (rc != LVB_OK) return rc;
   }
   if (rows > lvb::kv8::kMaxRows) {
     const dim3 grid(static_cast<unsigned>(max_query_len), static_cast<unsigned>(num_query_heads),
