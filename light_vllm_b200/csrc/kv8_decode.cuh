@@ -53,10 +53,15 @@ struct AttnArgs {
   int hq, group;
   bool query_vec, out_vec;  // rows allow 16-byte loads, 8-byte stores
   float scale_log2;  // softmax scale * log2(e)
-  // decode kernel
-  float *part_o;      // [2 * CTAs][kMaxRows][D]
-  float2 *part_ml;    // [2 * CTAs][kMaxRows]: m, L
-  uint32_t *counts;   // [num_seqs][hkv], zero between calls
+  int few_rows;      // requests of up to this many query rows are the decode kernel's
+  // Pieces of items that cross CTAs, and how many of an item's CTAs are done
+  // (kept at the CTA that the item begins in; zero between calls).
+  float *part_o;         // decode kernel: [2 * CTAs][kMaxRows][D]
+  float2 *part_ml;       // [2 * CTAs][kMaxRows]: m, L
+  uint32_t *counts;      // [CTAs]
+  float *tile_o;         // tile kernel: [2 * CTAs][kTileRows][D]
+  float2 *tile_ml;       // [2 * CTAs][kTileRows]
+  uint32_t *tile_counts;  // [CTAs]
 };
 
 // Two fp16 values of bytes 0, 1 (kHi: 2, 3) of four codes.
@@ -97,6 +102,12 @@ __device__ __forceinline__ float log2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void lds_16(uint32_t (&v)[4], uint32_t src) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
 }
@@ -106,6 +117,40 @@ __device__ __forceinline__ void lds_8(uint32_t (&v)[2], uint32_t src) {
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) { return pack2<false>(lo, hi); }
+
+// Eight elements of a row, one load where rows are 16-byte aligned.
+template <bool kBf16>
+__device__ __forceinline__ void load8(const uint16_t *src, bool some, bool vec, float (&x)[8]) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  uint16_t *e = reinterpret_cast<uint16_t *>(&v);
+  if (some && vec) {
+    v = *reinterpret_cast<const uint4 *>(src);
+  } else if (some) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = src[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_float<kBf16>(e[i]);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void store8(uint16_t *dst, bool vec, const float (&x)[8]) {
+  if (vec) {
+    *reinterpret_cast<uint4 *>(dst) =
+        make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]), pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[i] = from_float<kBf16>(x[i]);
+  }
+}
+
+// The power of two that brings `top` to [2^to, 2^(to + 1)), within the normal range.
+__device__ __forceinline__ float scale_to(float top, int to) {
+  const int field = static_cast<int>(__float_as_uint(top) >> 23);
+  return __uint_as_float(static_cast<uint32_t>(min(max(254 + to - field, 1), 254)) << 23);
+}
+
+__device__ __forceinline__ void named_barrier_256() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // A row of queries as fp16 times 2^shift (returned as 2^-shift): fp16 rows as
 // they are; bf16 rows with their largest element brought to [2^7, 2^8), which
@@ -120,9 +165,7 @@ __device__ __forceinline__ float query_shift(const float (&x)[N]) {
     for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // exponent field of 2^(7 - e): 127 + 7 - (field - 127), kept in the normal range
-    const int field = static_cast<int>(__float_as_uint(top) >> 23);
-    return __uint_as_float(static_cast<uint32_t>(min(max(261 - field, 1), 254)) << 23);
+    return scale_to(top, 7);
   }
 }
 
@@ -152,12 +195,6 @@ __device__ __forceinline__ void cp_async_8(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
-__device__ __forceinline__ float rcp_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <bool kBf16, bool kFp8, int D, int kNT>
 __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>::kCtasPerSm)
     decode_kernel(const __grid_constant__ AttnArgs a) {
@@ -183,7 +220,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   // Pages of request r's items (0: not this kernel's, or refused).
   auto request_pages = [&](int r) {
     int q0, n, c;
-    if (!request_range(s, r, q0, n, c) || n == 0 || n > kRows / a.group) return 0;
+    if (!request_range(s, r, q0, n, c) || n == 0 || n * a.group > a.few_rows) return 0;
     return (c + n + kPage - 1) / kPage;
   };
   // Exclusive prefix of a value over the CTA; `sum` is the total.
@@ -556,7 +593,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       // The CTAs that hold a piece of the item.
       const long long item = end - left - seg.first;
       const int c0 = static_cast<int>(item / run), c1 = static_cast<int>((item + seg.pages - 1) / run);
-      uint32_t *count = a.counts + static_cast<int64_t>(seg.r) * s.hkv + seg.kvh;
+      uint32_t *count = a.counts + c0;
       __threadfence();
       __syncthreads();
       if (tid == 0) last_sm = atomicAdd(count, 1u) == static_cast<uint32_t>(c1 - c0);

@@ -1,0 +1,619 @@
+// Attention of many query rows over the 8-bit paged cache (prompt chunks, long
+// verifications): tcgen05 with fp32 accumulators in tensor memory.
+//
+// An item is one request, one KV head and up to 256 of its query rows (row R is
+// token R / group, head R % group), taken as two tiles A and B of 128 rows that
+// share every K/V tile of 128 positions.  Roles of a CTA (one per SM):
+//   warps 0..3, 4..7  softmax of tile A, B: one thread for each row
+//   warps 8..11       converters: codes from global memory to registers one tile
+//                     ahead, to fp16 (exact for both formats), to shared memory
+//                     in the 128-byte-swizzled operand layouts (K: K-major, V:
+//                     MN-major as it lies), double-buffered
+//   warp 12           one thread issues the MMAs: S = Q K^T (both operands in
+//                     shared memory), O += P V (P in tensor memory)
+// While one tile's softmax runs, the tensor core works for the other.  P takes
+// the place of the first half of its own S.
+//
+// Mathematics as in the decode kernel: x_j = (q . key code_j) f_b + log2 w_b,
+// O = sum 2^(x_j - m) code_j, L = sum 2^(x_j - m) / w_b, out = O / L.  A row's
+// maximum of 16 positions of a block is taken over raw scores (f_b >= 0), so the
+// scales cost one multiply-add for 16.  Weights enter the second product as
+// fp16, times 2^8; O is rescaled in tensor memory only when m would grow by
+// more than 2^4 (kLazy).
+//
+// What bounds it: for each 256 x 128 scores 4 x 512 cycles of MMA, 2048 cycles of
+// exponentials (16 a cycle and SM), and about 7000 issue slots of 4 a cycle.
+//
+// Split.  K/V tiles of all items are laid end to end and cut into one equal run
+// for each CTA; items that cross a cut are joined by the last of their CTAs to
+// finish, in order (the decode kernel's scheme).
+#pragma once
+
+#include "kv8_decode.cuh"
+
+namespace lvb {
+namespace kv8 {
+
+constexpr int kTileRows = 256;  // query rows of an item
+constexpr int kTilePos = 128;   // positions of a K/V tile
+constexpr int kMinTiles = 2;    // K/V tiles of a CTA, at least
+
+// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
+__device__ __forceinline__ void umma_f16_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 codes to fp16.
+template <bool kFp8>
+__device__ __forceinline__ void codes_to_half(const uint4 &v, uint4 &lo, uint4 &hi) {
+  using P = Pair<kFp8>;
+  const uint32_t a = P::bias(v.x), b = P::bias(v.y), c = P::bias(v.z), d = P::bias(v.w);
+  lo = make_uint4(P::template get<false>(a), P::template get<true>(a), P::template get<false>(b), P::template get<true>(b));
+  hi = make_uint4(P::template get<false>(c), P::template get<true>(c), P::template get<false>(d), P::template get<true>(d));
+}
+
+template <int D>
+struct TileCfg {
+  static constexpr int kThreads = 13 * 32;
+  static constexpr int kQBytes = 128 * D * 2;        // one tile's queries
+  static constexpr int kSideBytes = kTilePos * D * 2;  // K (or V) of a K/V tile
+  static constexpr int kHalf = 128 * 128;            // 64 elements of 128 rows
+  static constexpr int kKOff = 2 * kQBytes;          // [2 stages]
+  static constexpr int kVOff = kKOff + 2 * kSideBytes;
+  static constexpr int kScaleOff = kVOff + 2 * kSideBytes;  // float4 [4][8]: key scale, log2 and inverse of the value scale
+  static constexpr int kBookOff = kScaleOff + 4 * 8 * 16;
+  static constexpr int kSmemBytes = 1024 + kBookOff + 512;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+};
+
+// One run of K/V tiles of one item.
+struct TileSegment {
+  int r, kvh, tile;     // rows [256 tile, ..)
+  int first, last;      // K/V tiles [first, last)
+  int units;            // of the whole item
+  int q0, n, computed;  // the request's
+  int rows;             // of this item
+};
+
+template <bool kBf16, bool kFp8, int D>
+__global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __grid_constant__ AttnArgs a) {
+  using Cfg = TileCfg<D>;
+  constexpr float kNone = -1e30f;
+  constexpr float kHead = 8.f, kLazy = 4.f;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float4 *scale_sm = reinterpret_cast<float4 *>(smem + Cfg::kScaleOff);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kBookOff);
+  uint64_t *k_full = bars, *v_full = bars + 2, *k_empty = bars + 4, *v_empty = bars + 6, *sc_full = bars + 8,
+           *s_full = bars + 12, *p_full = bars + 14, *o_done = bars + 16, *q_full = bars + 18;
+  long long *scan = reinterpret_cast<long long *>(bars + 20);  // [13]
+  long long *start_units = scan + 13;
+  uint32_t *tmem_sm = reinterpret_cast<uint32_t *>(start_units + 1);
+  int *start_request = reinterpret_cast<int *>(tmem_sm + 1);
+  int *last_sm = start_request + 1;  // [2]
+  volatile int *abort_flag = last_sm + 2;
+
+  pdl_wait();
+  const Step &s = a.step;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  // K/V tiles of the rows [256 i, 256 i + 256) of a request of n tokens.
+  auto item_units = [&](int n, int computed, int i) {
+    const int tok = (min(n * a.group, (i + 1) * kTileRows) - 1) / a.group;
+    return (computed + tok + kTilePos) / kTilePos;
+  };
+  auto num_tiles = [&](int n) { return (n * a.group + kTileRows - 1) / kTileRows; };
+  // K/V tiles of one KV head of request r (0: the decode kernel's, or refused).
+  auto request_units = [&](int r) {
+    int q0, n, c;
+    long long sum = 0;
+    if (request_range(s, r, q0, n, c) && n * a.group > a.few_rows)
+      for (int i = 0; i < num_tiles(n); ++i) sum += item_units(n, c, i);
+    return sum;
+  };
+  auto block_scan = [&](long long v, long long &sum) {
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    long long before = 0;
+    sum = 0;
+    for (int w = 0; w < 13; ++w) {
+      if (w < warp) before += scan[w];
+      sum += scan[w];
+    }
+    return before + x - v;
+  };
+  long long total = 0, mine = 0, sum = 0, ex = 0;
+  for (int base = 0; base < s.num_seqs; base += Cfg::kThreads) {
+    mine = base + tid < s.num_seqs ? request_units(base + tid) : 0;
+    ex = block_scan(mine, sum);
+    total += sum * s.hkv;
+  }
+  long long run = (total + gridDim.x - 1) / gridDim.x;
+  if (run < kMinTiles) run = kMinTiles;
+  const long long begin = run * blockIdx.x;
+  if (begin >= total) return;
+  const long long end = begin + run < total ? begin + run : total;
+  {
+    long long before = 0;
+    for (int base = 0; base < s.num_seqs; base += Cfg::kThreads) {
+      if (s.num_seqs > Cfg::kThreads) {
+        mine = base + tid < s.num_seqs ? request_units(base + tid) : 0;
+        ex = block_scan(mine, sum);
+      }
+      const long long lo = before + ex * s.hkv, hi = lo + mine * s.hkv;
+      if (lo <= begin && begin < hi) {
+        *start_request = base + tid;
+        *start_units = lo;
+      }
+      before += sum * s.hkv;
+    }
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_sm, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + i, 4);
+      mbar_init(v_full + i, 4);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_done + i, 1);
+      mbar_init(q_full + i, 4);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(sc_full + i, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_sm;
+
+  auto describe = [&](int r, int kvh, int tile, int first, long long left, TileSegment &seg) {
+    seg.r = r;
+    seg.kvh = kvh;
+    seg.tile = tile;
+    seg.q0 = s.qsl[r];
+    seg.n = s.qsl[r + 1] - seg.q0;
+    seg.computed = s.computed[r];
+    seg.rows = min(kTileRows, seg.n * a.group - tile * kTileRows);
+    seg.units = item_units(seg.n, seg.computed, tile);
+    seg.first = first;
+    seg.last = left < seg.units - first ? first + static_cast<int>(left) : seg.units;
+  };
+  TileSegment seg;
+  long long left = end - begin;  // K/V tiles of the run from the present segment on
+  {
+    const int r = *start_request;
+    const long long per_head = request_units(r);
+    long long inside = begin - *start_units;
+    const int kvh = static_cast<int>(inside / per_head);
+    inside -= kvh * per_head;
+    const int c = s.computed[r], n = s.qsl[r + 1] - s.qsl[r];
+    int tile = 0;
+    while (inside >= item_units(n, c, tile)) inside -= item_units(n, c, tile++);
+    describe(r, kvh, tile, static_cast<int>(inside), left, seg);
+  }
+  // To the run's next segment; false at its end.
+  auto advance = [&]() {
+    left -= seg.last - seg.first;
+    if (left <= 0) return false;
+    int r = seg.r, kvh = seg.kvh, tile = seg.tile + 1;
+    if (tile == num_tiles(seg.n)) {
+      tile = 0;
+      if (++kvh == s.hkv) {
+        kvh = 0;
+        do {
+          ++r;
+        } while (request_units(r) == 0);  // tiles are left, so a request is
+      }
+    }
+    describe(r, kvh, tile, 0, left, seg);
+    return true;
+  };
+
+  TileSegment joins[2];  // pieces of items that other CTAs hold pieces of
+  long long join_item[2];
+  int num_joins = 0;
+  bool ok = true, more = true;
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------- converters ----------------
+    constexpr int kChunks = D / 16;            // 16-byte pieces of a row
+    constexpr int kRowsPass = 128 / kChunks;   // rows that the 128 threads take at a time
+    constexpr int kPasses = kTilePos / kRowsPass;
+    const int ct = tid - 256, c = ct % kChunks, row0 = ct / kChunks;
+    const int ppb = s.bs / kPage;
+    const uint32_t head_bytes = static_cast<uint32_t>(s.bs) * D;
+    uint32_t h_page = 0, in_page = 0;  // lane i < 8: page i's head and place in its block
+    uint4 kreg[kPasses], vreg[kPasses];
+    float ksc = 0.f, vsc = 1.f;
+    // Where a tile's pages are.
+    auto locate = [&](const TileSegment &of, int tile) {
+      const int p = tile * (kTilePos / kPage) + (lane & 7);
+      const int pages = (of.computed + of.n + kPage - 1) / kPage;
+      int phys = p < pages ? s.tables[of.r * s.table_stride + (ppb == 1 ? p : p / ppb)] : 0;
+      if (static_cast<uint32_t>(phys) >= static_cast<uint32_t>(s.num_blocks)) {
+        record_device_error(LVB_DEVERR_INDEX);
+        phys = -1;
+      }
+      h_page = p >= pages || phys < 0 ? ~0u : static_cast<uint32_t>(phys) * s.hkv + of.kvh;
+      in_page = ppb == 1 ? 0u : static_cast<uint32_t>(p % ppb) * (kPage * D);
+      ksc = vsc = 0.f;
+      if (h_page != ~0u) ksc = __ldg(a.key_scales + h_page), vsc = __ldg(a.value_scales + h_page);
+    };
+    auto load = [&](const TileSegment &of, int tile, const uint8_t *codes, uint4 (&reg)[kPasses]) {
+      const int stop = of.computed + of.n;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int row = i * kRowsPass + row0;
+        const uint32_t h = __shfl_sync(0xffffffffu, h_page, row / kPage);
+        const uint64_t at = static_cast<uint64_t>(h) * head_bytes + __shfl_sync(0xffffffffu, in_page, row / kPage) +
+                            (row % kPage) * D + c * 16;
+        // zeros past the end: 0 times what a stale slot holds may be NaN
+        reg[i] = make_uint4(0, 0, 0, 0);
+        if (h != ~0u && tile * kTilePos + row < stop) reg[i] = __ldg(reinterpret_cast<const uint4 *>(codes + at));
+      }
+    };
+    // Registers to a stage's operand rows.
+    auto convert = [&](uint8_t *dst, const uint4 (&reg)[kPasses]) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int row = i * kRowsPass + row0;
+        uint4 lo, hi;
+        codes_to_half<kFp8>(reg[i], lo, hi);
+        uint8_t *base = dst + (c >> 2) * Cfg::kHalf + row * 128;
+        *reinterpret_cast<uint4 *>(base + ((((2 * c) & 7) ^ (row & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4 *>(base + ((((2 * c + 1) & 7) ^ (row & 7)) << 4)) = hi;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    int g = 0;  // K/V tiles so far
+    locate(seg, seg.first);
+    load(seg, seg.first, a.key_codes, kreg);
+    load(seg, seg.first, a.value_codes, vreg);
+    while (more) {
+      const TileSegment now = seg;
+      more = advance();
+      for (int t = now.first; t < now.last; ++t, ++g) {
+        const int st = g & 1;
+        const bool same = t + 1 < now.last;
+        if (warp == 8) {
+          if (lane < 8) {
+            const float vw = vsc > 0.f ? vsc : 1.f;
+            // a page that does not exist weighs nothing
+            scale_sm[(g & 3) * 8 + lane] =
+                h_page == ~0u ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(ksc, log2_fast(vw), rcp_fast(vw), 0.f);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sc_full + (g & 3));
+        }
+        if (g >= 2) ok = ok && mbar_wait(k_empty + st, ((g >> 1) - 1) & 1, abort_flag);
+        convert(smem + Cfg::kKOff + st * Cfg::kSideBytes, kreg);
+        if (lane == 0) mbar_arrive(k_full + st);
+        if (same || more) {
+          locate(same ? now : seg, same ? t + 1 : seg.first);
+          load(same ? now : seg, same ? t + 1 : seg.first, a.key_codes, kreg);
+        }
+        if (g >= 2) ok = ok && mbar_wait(v_empty + st, ((g >> 1) - 1) & 1, abort_flag);
+        convert(smem + Cfg::kVOff + st * Cfg::kSideBytes, vreg);
+        if (lane == 0) mbar_arrive(v_full + st);
+        if (same || more) load(same ? now : seg, same ? t + 1 : seg.first, a.value_codes, vreg);
+      }
+    }
+  } else if (warp == 12) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t kIdescS = umma_idesc_f16(128, kTilePos, 0, 0, 0, 0);
+      constexpr uint32_t kIdescO = umma_idesc_f16(128, D, 0, 0, 0, 1);
+      constexpr int kKSteps = D / 16;
+      const uint32_t base = smem_u32(smem);
+      int g = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      while (more && ok) {
+        const int tiles = seg.rows > 128 ? 2 : 1;
+        const int count = seg.last - seg.first;
+        auto scores = [&](int x, int st) {
+          const uint64_t q_desc = umma_smem_desc_sw128(base + x * Cfg::kQBytes, 16, 1024);
+          const uint64_t k_desc = umma_smem_desc_sw128(base + Cfg::kKOff + st * Cfg::kSideBytes, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < kKSteps; ++k) {
+            const uint64_t off = (k >> 2) * (Cfg::kHalf >> 4) + (k & 3) * 2;
+            umma_f16(tmem + x * 128, q_desc + off, k_desc + off, kIdescS, k > 0);
+          }
+          umma_commit(s_full + x);
+        };
+        for (int x = 0; x < tiles && ok; ++x) ok = mbar_wait(q_full + x, q_phase[x]++ & 1, abort_flag);
+        ok = ok && mbar_wait(k_full + (g & 1), (g >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        for (int x = 0; x < tiles; ++x) scores(x, g & 1);
+        umma_commit(k_empty + (g & 1));
+        for (int t = 0; t < count && ok; ++t, ++g) {
+          const int st = g & 1;
+          const bool next = t + 1 < count;
+          ok = mbar_wait(v_full + st, (g >> 1) & 1, abort_flag);
+          for (int x = 0; x < tiles && ok; ++x) {
+            ok = mbar_wait(p_full + x, p_phase[x]++ & 1, abort_flag);
+            if (ok && x == 0 && next) ok = mbar_wait(k_full + (st ^ 1), ((g + 1) >> 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t v_desc = umma_smem_desc_sw128(base + Cfg::kVOff + st * Cfg::kSideBytes, Cfg::kHalf, 1024);
+#pragma unroll
+            for (int k = 0; k < kTilePos / 16; ++k)
+              umma_f16_tmem_a(tmem + 256 + x * 128, tmem + x * 128 + k * 8, v_desc + k * 128, kIdescO, t > 0 || k > 0);
+            umma_commit(o_done + x);
+            if (next) scores(x, st ^ 1);
+          }
+          if (!ok) break;
+          umma_commit(v_empty + st);
+          if (next) umma_commit(k_empty + (st ^ 1));
+        }
+        more = advance();
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax ----------------
+    const int x = warp >> 2;           // tile A or B
+    const int row_in = tid & 127;      // row of the tile = tensor memory lane
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    const uint32_t t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
+    int g = 0, phase = 0;  // K/V tiles of the CTA, and of this tile
+    while (more) {
+      const int rows = seg.rows - x * 128;
+      if (rows > 0) {
+        // This row's queries, brought to fp16 by a power of two where they are bf16.
+        const int row = seg.tile * kTileRows + x * 128 + row_in;
+        const bool some = row_in < rows;
+        const int tok = some ? row / a.group : 0, head = some ? row - tok * a.group : 0;
+        const uint16_t *src = a.query + (seg.q0 + tok) * a.query_stride + (seg.kvh * a.group + head) * D;
+        float up = a.scale_log2 < 0.f ? -1.f : 1.f;
+        if constexpr (kBf16) {
+          float top = 0.f;
+          for (int d = 0; d < D; d += 8) {
+            float e[8];
+            load8<kBf16>(src + d, some, a.query_vec, e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(e[i]));
+          }
+          up *= scale_to(top, 7);
+        }
+        const float fr = a.scale_log2 / up;
+        uint8_t *dst = smem + x * Cfg::kQBytes + row_in * 128;
+        for (int d = 0; d < D; d += 8) {
+          float e[8];
+          load8<kBf16>(src + d, some, a.query_vec, e);
+          const uint4 v = make_uint4(pack2<false>(e[0] * up, e[1] * up), pack2<false>(e[2] * up, e[3] * up),
+                                     pack2<false>(e[4] * up, e[5] * up), pack2<false>(e[6] * up, e[7] * up));
+          *reinterpret_cast<uint4 *>(dst + (d >> 6) * Cfg::kHalf + ((((d >> 3) & 7) ^ (row_in & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full + x);
+
+        const int limit = some ? seg.computed + tok : -1;  // last position that the row sees
+        const bool idle = (warp & 3) * 32 >= rows;  // none of the warp's rows exists
+        float m = kNone, l = 0.f;
+        for (int t = seg.first; t < seg.last; ++t, ++g, ++phase) {
+          ok = ok && mbar_wait(sc_full + (g & 3), (g >> 2) & 1, abort_flag);
+          ok = ok && mbar_wait(s_full + x, phase & 1, abort_flag);
+          if (idle) {
+            if (lane == 0) mbar_arrive(p_full + x);
+            continue;
+          }
+          tc_fence_after();
+          const float4 *scales = scale_sm + (g & 3) * 8;
+          const int seen = limit - t * kTilePos;  // positions 0 .. seen of the tile are visible
+          const bool masked = __any_sync(0xffffffffu, seen < kTilePos - 1);
+          float top = kNone;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld_x32(t_s + c * 32, v);
+            tmem_wait_ld();
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i > seen) v[i] = 0xff800000u;  // -inf
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float mx = __uint_as_float(v[h * 16]);
+#pragma unroll
+              for (int i = 1; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(v[h * 16 + i]));
+              const float4 sc = scales[c * 2 + h];
+              if (mx > -INFINITY) top = fmaxf(top, fmaf(mx, fr * sc.x, sc.y));  // (-inf * 0 is no maximum)
+            }
+          }
+          // O is rescaled when the maximum grows by more than kLazy.
+          const bool first = t == seg.first;
+          if (__any_sync(0xffffffffu, top > m + kLazy)) {
+            const float now = fmaxf(m, top);
+            const float alpha = exp2_fast(m - now);
+            m = now;
+            l *= alpha;
+            if (!first) {
+              ok = ok && mbar_wait(o_done + x, (phase - 1) & 1, abort_flag);
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld_x32(t_o + c * 32, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                tmem_st_x32(t_o + c * 32, v);
+              }
+            }
+          }
+          const float base = m - kHead;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], pk[16];
+            tmem_ld_x32(t_s + c * 32, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 sc = scales[c * 2 + h];
+              const float fk = fr * sc.x, add = sc.y - base;
+              float part = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                float e0 = exp2_fast(fmaf(__uint_as_float(v[h * 16 + i]), fk, add));
+                float e1 = exp2_fast(fmaf(__uint_as_float(v[h * 16 + i + 1]), fk, add));
+                if (masked) {
+                  if (c * 32 + h * 16 + i > seen) e0 = 0.f;
+                  if (c * 32 + h * 16 + i + 1 > seen) e1 = 0.f;
+                }
+                part += e0 + e1;
+                pk[h * 8 + i / 2] = pack2<false>(e0, e1);
+              }
+              l = fmaf(part, sc.z, l);
+            }
+            tmem_st_x16(t_s + c * 16, pk);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full + x);
+        }
+        // The item's (or piece's) result.
+        ok = ok && mbar_wait(o_done + x, (phase - 1) & 1, abort_flag);
+        tc_fence_after();
+        const bool whole = seg.first == 0 && seg.last == seg.units;
+        const int64_t piece = (2 * blockIdx.x + (seg.first == 0 ? 1 : 0)) * static_cast<int64_t>(kTileRows) + x * 128 + row_in;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t *out = a.out + (seg.q0 + tok) * a.out_stride + (seg.kvh * a.group + head) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld_x32(t_o + c * 32, v);
+          tmem_wait_ld();
+          if (!some || !ok) continue;
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float e[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) e[k] = __uint_as_float(v[i + k]) * inv;
+              store8<kBf16>(out + c * 32 + i, a.out_vec, e);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4 *>(a.tile_o + piece * D + c * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        }
+        if (!whole) a.tile_ml[piece] = make_float2(m, some ? l : 0.f);
+        tc_fence_before();
+      } else {
+        g += seg.last - seg.first;
+      }
+      if (!(seg.first == 0 && seg.last == seg.units)) {
+        joins[num_joins] = seg;
+        join_item[num_joins++] = end - left - seg.first;
+      }
+      more = advance();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+  if (tid >= 256) return;
+
+  // Items that other CTAs hold pieces of: whoever finishes an item last adds its pieces up, in order.
+  __threadfence();
+  named_barrier_256();
+  for (int i = 0; i < num_joins; ++i) {
+    const TileSegment &j = joins[i];
+    const int c0 = static_cast<int>(join_item[i] / run), c1 = static_cast<int>((join_item[i] + j.units - 1) / run);
+    if (tid == 0) last_sm[i] = atomicAdd(a.tile_counts + c0, 1u) == static_cast<uint32_t>(c1 - c0);
+  }
+  named_barrier_256();
+  __threadfence();
+  for (int i = 0; i < num_joins; ++i) {
+    if (!last_sm[i]) continue;
+    const TileSegment &j = joins[i];
+    const int c0 = static_cast<int>(join_item[i] / run), c1 = static_cast<int>((join_item[i] + j.units - 1) / run);
+    if (tid == 0) a.tile_counts[c0] = 0;
+    for (int k = tid; k < j.rows * (D / 8); k += 256) {
+      const int row = k / (D / 8), d = (k - row * (D / 8)) * 8;
+      float top = kNone;
+      for (int c = c0; c <= c1; ++c)
+        top = fmaxf(top, __ldcg(a.tile_ml + static_cast<int64_t>(2 * c + (c == c0)) * kTileRows + row).x);
+      float sum_l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int c = c0; c <= c1; ++c) {
+        const int64_t at = static_cast<int64_t>(2 * c + (c == c0)) * kTileRows + row;
+        const float2 ml = __ldcg(a.tile_ml + at);
+        const float wt = exp2_fast(ml.x - top);
+        sum_l = fmaf(wt, ml.y, sum_l);
+        const float4 u = __ldcg(reinterpret_cast<const float4 *>(a.tile_o + at * D + d));
+        const float4 w = __ldcg(reinterpret_cast<const float4 *>(a.tile_o + at * D + d + 4));
+        acc[0] = fmaf(wt, u.x, acc[0]), acc[1] = fmaf(wt, u.y, acc[1]), acc[2] = fmaf(wt, u.z, acc[2]);
+        acc[3] = fmaf(wt, u.w, acc[3]), acc[4] = fmaf(wt, w.x, acc[4]), acc[5] = fmaf(wt, w.y, acc[5]);
+        acc[6] = fmaf(wt, w.z, acc[6]), acc[7] = fmaf(wt, w.w, acc[7]);
+      }
+      const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= inv;
+      const int abs_row = j.tile * kTileRows + row;
+      const int tok = abs_row / a.group, head = abs_row - tok * a.group;
+      store8<kBf16>(a.out + (j.q0 + tok) * a.out_stride + (j.kvh * a.group + head) * D + d, a.out_vec, acc);
+    }
+  }
+}
+
+}  // namespace kv8
+}  // namespace lvb

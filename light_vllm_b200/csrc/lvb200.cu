@@ -27,8 +27,9 @@
 #include "awq_decode.cuh"
 #include "awq_i8.cuh"
 #include "allreduce.cuh"
-#include "kv8_attention.cuh"
 #include "kv8_cache.cuh"
+#include "kv8_decode.cuh"
+#include "kv8_tiles.cuh"
 #include "lvb_common.cuh"
 #include "paged_attention.cuh"
 #include "spec_verify.cuh"
@@ -2225,26 +2226,52 @@ int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, const fl
 
 namespace {
 
-// Workspace of an attention call: partial sums for two pieces of each CTA that
-// the decode kernel may run, then the item counters.  The counters' place is
-// the same for every call on a device, so that they stay zero whatever calls
-// share a buffer.
+// Workspace of an attention call: the CTAs' counters first, at the same place
+// for every call on a device, so that they stay zero whatever calls share a
+// buffer; then two pieces for each CTA of the decode kernel, and, where a
+// request may have more rows than that takes, of the tile kernel.
 struct Kv8Workspace {
-  size_t o, ml, counts;  // offsets
+  size_t counts, tile_counts, o, ml, tile_o, tile_ml, total;  // offsets
 };
 
-Kv8Workspace kv8_workspace(int sms) {
-  constexpr int kMaxCtasPerSm = 2;
-  const size_t slots = static_cast<size_t>(2) * kMaxCtasPerSm * sms * lvb::kv8::kMaxRows;
+constexpr int kKv8DecodeCtasPerSm = 2;
+
+// Query rows of one KV head that the decode kernel takes: of every request if
+// the longest fits, else of single tokens beside prompt chunks.
+int kv8_few_rows(int64_t max_query_len, int64_t group) {
+  const int64_t rows = max_query_len * group;
+  const int64_t fit = rows <= lvb::kv8::kMaxRows ? rows : group;
+  return fit <= 8 ? 8 : fit <= lvb::kv8::kMaxRows ? lvb::kv8::kMaxRows : 0;
+}
+
+Kv8Workspace kv8_workspace(int sms, bool tiles) {
+  const size_t ctas = static_cast<size_t>(sms) * kKv8DecodeCtasPerSm;
+  const size_t rows = 2 * ctas * lvb::kv8::kMaxRows, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
   Kv8Workspace w{};
-  w.ml = w.o + slots * 128 * sizeof(float);
-  w.counts = round256(w.ml + slots * sizeof(float2));
+  w.tile_counts = round256(ctas * 4);
+  w.o = w.tile_counts + round256(static_cast<size_t>(sms) * 4);
+  w.ml = w.o + rows * 128 * sizeof(float);
+  w.tile_o = round256(w.ml + rows * sizeof(float2));
+  w.tile_ml = w.tile_o + tile_rows * 128 * sizeof(float);
+  w.total = round256(w.tile_ml + tile_rows * sizeof(float2));
   return w;
+}
+
+template <bool kBf16, bool kFp8, int D>
+int launch_kv8_tiles(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) {
+  using Cfg = lvb::kv8::TileCfg<D>;
+  static bool smem_done[kMaxDevices] = {false};
+  auto kernel = lvb::kv8::tile_kernel<kBf16, kFp8, D>;
+  int rc = ensure_smem(kernel, Cfg::kSmemBytes, dev, smem_done);
+  if (rc != LVB_OK) return rc;
+  cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(sm_count(dev))), dim3(Cfg::kThreads), Cfg::kSmemBytes, stream, a);
+  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 tile_kernel launch");
 }
 
 template <bool kBf16, bool kFp8, int D, int kNT>
 int launch_kv8_decode(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) {
   using Cfg = lvb::kv8::DecodeCfg<D, kNT>;
+  static_assert(Cfg::kCtasPerSm <= kKv8DecodeCtasPerSm, "workspace");
   static bool smem_done[kMaxDevices] = {false};
   auto kernel = lvb::kv8::decode_kernel<kBf16, kFp8, D, kNT>;
   int rc = ensure_smem(kernel, Cfg::kSmemBytes, dev, smem_done);
@@ -2258,10 +2285,13 @@ int launch_kv8_decode(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream)
 
 size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
                                          int64_t head_size, int64_t max_query_len, int64_t max_seq_len) {
-  (void)num_query_heads, (void)head_size, (void)max_query_len, (void)max_seq_len;
+  (void)head_size, (void)max_seq_len;
   int dev = 0;
-  if (num_seqs <= 0 || num_kv_heads <= 0 || current_device(&dev) != LVB_OK) return 0;
-  return round256(kv8_workspace(sm_count(dev)).counts + static_cast<size_t>(num_seqs) * num_kv_heads * 4);
+  if (num_seqs <= 0 || num_kv_heads <= 0 || num_query_heads <= 0 || max_query_len <= 0 || max_query_len > INT_MAX ||
+      current_device(&dev) != LVB_OK)
+    return 0;
+  const int64_t group = num_query_heads / num_kv_heads;
+  return kv8_workspace(sm_count(dev), max_query_len * group > kv8_few_rows(max_query_len, group)).total;
 }
 
 int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
@@ -2296,40 +2326,34 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
   a.hq = static_cast<int>(num_query_heads);
   a.group = static_cast<int>(num_query_heads / num_kv_heads);
   a.query_vec = aligned16(query) && query_token_stride % 8 == 0;
-  a.out_vec = (reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_token_stride % 4 == 0;
+  a.out_vec = aligned16(out) && out_token_stride % 8 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
+  if (max_query_len * a.group > INT_MAX) return fail(LVB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
   int dev = 0;
   rc = current_device(&dev);
   if (rc != LVB_OK) return rc;
-  const int sms = sm_count(dev);
-  const Kv8Workspace w = kv8_workspace(sms);
-  const size_t need = w.counts + static_cast<size_t>(num_seqs) * num_kv_heads * 4;
-  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
-    return fail(LVB_ERR_WORKSPACE, "kv8_attention: workspace of %zu bytes is below the %zu required", workspace_bytes, need);
+  a.few_rows = kv8_few_rows(max_query_len, a.group);
+  const bool tiles = max_query_len * a.group > a.few_rows;
+  const Kv8Workspace w = kv8_workspace(sm_count(dev), tiles);
+  if (workspace == nullptr || workspace_bytes < w.total || !aligned16(workspace))
+    return fail(LVB_ERR_WORKSPACE, "kv8_attention: workspace of %zu bytes is below the %zu required", workspace_bytes, w.total);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
+  a.counts = reinterpret_cast<uint32_t *>(ws + w.counts);
+  a.tile_counts = reinterpret_cast<uint32_t *>(ws + w.tile_counts);
   a.part_o = reinterpret_cast<float *>(ws + w.o);
   a.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
-  a.counts = reinterpret_cast<uint32_t *>(ws + w.counts);
+  a.tile_o = reinterpret_cast<float *>(ws + w.tile_o);
+  a.tile_ml = reinterpret_cast<float2 *>(ws + w.tile_ml);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t rows = max_query_len * a.group;
-  cudaError_t e = cudaSuccess;
-  if (a.group <= lvb::kv8::kMaxRows) {
-    rc = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
-      constexpr bool kB16 = decltype(b16)::value, kFp8 = decltype(fp8)::value;
-      return rows <= 8 ? launch_kv8_decode<kB16, kFp8, decltype(d)::value, 1>(a, dev, st)
-                       : launch_kv8_decode<kB16, kFp8, decltype(d)::value, 2>(a, dev, st);
-    });
-    if (rc != LVB_OK) return rc;
-  }
-  if (rows > lvb::kv8::kMaxRows) {
-    const dim3 grid(static_cast<unsigned>(max_query_len), static_cast<unsigned>(num_query_heads),
-                    static_cast<unsigned>(num_seqs));
-    e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
-      return launch_pdl(lvb::kv8::attention_kernel<decltype(b16)::value, decltype(fp8)::value, decltype(d)::value>, grid,
-                        dim3(32), 0, st, a);
-    });
-  }
-  return e == cudaSuccess ? LVB_OK : cuda_fail(e, "kv8 attention_kernel launch");
+  return kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
+    constexpr bool kB16 = decltype(b16)::value, kFp8 = decltype(fp8)::value;
+    constexpr int kD = decltype(d)::value;
+    int status = LVB_OK;
+    if (tiles) status = launch_kv8_tiles<kB16, kFp8, kD>(a, dev, st);
+    if (status == LVB_OK && a.few_rows == 8) status = launch_kv8_decode<kB16, kFp8, kD, 1>(a, dev, st);
+    if (status == LVB_OK && a.few_rows == 16) status = launch_kv8_decode<kB16, kFp8, kD, 2>(a, dev, st);
+    return status;
+  });
 }
 
 size_t lvb_verify_drafts_workspace_bytes(int64_t num_seqs, int64_t vocab_size) {
