@@ -19,6 +19,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblvb200.so"
 HOSTPACK_PATH = Path(__file__).resolve().parent / "_lib" / ("_hostpack" + sysconfig.get_config_var("EXT_SUFFIX"))
+TORCH_OPS_PATH = HOSTPACK_PATH.with_name("_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
 ABI_VERSION = 9
 
 LVB_OK = 0
@@ -220,6 +221,26 @@ def hostpack():
     module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                   for name in ("lvb_paged_kv_write", "lvb_paged_attention", "lvb_stage_step_metadata",
                                "lvb_paged_attention_kv")))
+    return module
+
+
+@functools.lru_cache(maxsize=1)
+def torch_ops():
+    """The CPython module that calls the operators straight from torch tensors."""
+
+    import torch  # noqa: F401 -- the module links against torch's libraries
+
+    if not TORCH_OPS_PATH.is_file():
+        raise NativeLibraryError(f"{TORCH_OPS_PATH} is not built; run `python -m light_vllm_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("light_vllm_b200._torch_ops", str(TORCH_OPS_PATH))
+    spec = importlib.util.spec_from_file_location("light_vllm_b200._torch_ops", str(TORCH_OPS_PATH), loader=loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    lib = library()
+    module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                  for name in ("lvb_kv8_append", "lvb_kv8_read_blocks", "lvb_kv8_attention",
+                               "lvb_kv8_attention_workspace_bytes", "lvb_verify_drafts",
+                               "lvb_verify_drafts_workspace_bytes")))
     return module
 
 

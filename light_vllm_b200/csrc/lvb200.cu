@@ -2357,8 +2357,8 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
 }
 
 size_t lvb_verify_drafts_workspace_bytes(int64_t num_seqs, int64_t vocab_size) {
-  (void)num_seqs, (void)vocab_size;
-  return 0;
+  (void)vocab_size;
+  return num_seqs > 0 ? static_cast<size_t>(num_seqs) * lvb::spec::kScratchWords * 8 : 0;
 }
 
 int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const float *draft_probs, int64_t draft_stride,
@@ -2366,8 +2366,7 @@ int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const fl
                       const int32_t *query_start_loc, int64_t *out_tokens, int32_t *num_accepted, int64_t num_seqs,
                       int64_t num_rows, int64_t max_query_len, int64_t vocab_size, void *workspace,
                       size_t workspace_bytes, lvb_stream_t stream) {
-  (void)workspace, (void)workspace_bytes;
-  if (num_seqs < 0 || num_seqs > INT_MAX || num_rows < 0 || num_rows > INT_MAX || max_query_len < 0 ||
+  if (num_seqs < 0 || num_seqs > 65535 || num_rows < 0 || num_rows > INT_MAX || max_query_len < 0 ||
       max_query_len > INT_MAX || vocab_size <= 0 || vocab_size > INT_MAX)
     return fail(LVB_ERR_INVALID, "verify_drafts: invalid batch or vocabulary size");
   if (num_seqs == 0) return LVB_OK;
@@ -2392,7 +2391,24 @@ int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const fl
   a.num_rows = static_cast<int>(num_rows);
   a.width = static_cast<int>(max_query_len);
   a.vocab = static_cast<int>(vocab_size);
-  cudaError_t e = launch_pdl(lvb::spec::verify_kernel, dim3(static_cast<unsigned>(num_seqs)),
-                             dim3(lvb::spec::kVerifyThreads), 0, reinterpret_cast<cudaStream_t>(stream), a);
+  const size_t need = lvb_verify_drafts_workspace_bytes(num_seqs, vocab_size);
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+    return fail(LVB_ERR_WORKSPACE, "verify_drafts: workspace of %zu bytes is below the %zu required", workspace_bytes, need);
+  a.scratch = static_cast<unsigned long long *>(workspace);
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc != LVB_OK) return rc;
+  // About eight CTAs of 256 threads for each SM, and chunks of at least 2048
+  // values (two loads of 16 bytes a thread).
+  const bool vec = vocab_size % 4 == 0 && target_stride % 4 == 0 && aligned16(target_probs) &&
+                   (!draft_probs || (draft_stride % 4 == 0 && aligned16(draft_probs)));
+  int64_t chunks = std::max<int64_t>(1, 8LL * sm_count(dev) / num_seqs);
+  chunks = std::min<int64_t>({chunks, (vocab_size + 2047) / 2048, lvb::spec::kMaxChunks});
+  const int64_t chunk = ((vocab_size + chunks - 1) / chunks + 3) / 4 * 4;
+  a.chunk = static_cast<int>(chunk);
+  const dim3 grid(static_cast<unsigned>((vocab_size + chunk - 1) / chunk), static_cast<unsigned>(num_seqs));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = vec ? launch_pdl(lvb::spec::verify_kernel<true>, grid, dim3(lvb::spec::kVerifyThreads), 0, st, a)
+                      : launch_pdl(lvb::spec::verify_kernel<false>, grid, dim3(lvb::spec::kVerifyThreads), 0, st, a);
   return e == cudaSuccess ? LVB_OK : cuda_fail(e, "verify_kernel launch");
 }

@@ -17,7 +17,9 @@ bytes of the 16-bit cache (runtime/execution/paged_cache.py:30-338, which has no
   step handler run over the 8-bit cache unchanged.
 
 All of it runs on the current stream, allocates through torch and does not
-synchronise.
+synchronise.  A call goes through ``_torch_ops`` (``csrc/torch_ops.cpp``), which
+checks and launches the usual case; the functions below hold every rule and
+message and take whatever that hands back.
 """
 
 from __future__ import annotations
@@ -118,7 +120,8 @@ class _Workspaces:
     needs it, and calls on one stream follow one another.  A grown buffer keeps
     its predecessors, which a captured graph may still name."""
 
-    def __init__(self) -> None:
+    def __init__(self, op: int) -> None:
+        self._op = op
         self._current: dict[tuple[int, int], Tensor] = {}
         self._kept: list[Tensor] = []
 
@@ -135,10 +138,19 @@ class _Workspaces:
                 self._kept.append(buf)
             buf = torch.zeros(max(1 << 20, 1 << (need - 1).bit_length()), dtype=torch.uint8, device=device)
             self._current[key] = buf
+            _native.torch_ops().set_scratch(self._op, device.index, stream, buf.data_ptr(), buf.numel())
         return buf.data_ptr(), buf.numel()
 
 
-_workspaces = _Workspaces()
+_workspaces = _Workspaces(0)
+_fast = None  # _torch_ops, loaded by the first call
+
+
+def _ops():
+    global _fast
+    if _fast is None:
+        _fast = _native.torch_ops()
+    return _fast
 
 
 def kv8_append(query: Tensor | None, key: Tensor, value: Tensor, layer: KV8Layer, step: KV8Step, *,
@@ -154,6 +166,11 @@ def kv8_append(query: Tensor | None, key: Tensor, value: Tensor, layer: KV8Layer
     None.  ``query_out`` (``query`` itself, if wanted) receives the rotated
     queries instead of a new tensor."""
 
+    done = (_fast or _ops()).kv8_append(query, key, value, *layer, *step, positions, cos, sin, query_out)
+    if done is not None:
+        if type(done) is int:
+            _native.check(done, "lvb_kv8_append")
+        return None if done is True else done
     code = _check_layer(layer)
     keys = layer.keys
     num_blocks, hkv, block, d = keys.shape
@@ -210,8 +227,14 @@ def kv8_read_blocks(layer: KV8Layer, block_ids: Tensor, *, dtype: torch.dtype) -
     """Keys and values [n, kv_heads, block_size, head_size] of the blocks
     ``block_ids`` (int32 on the cache's device) in ``dtype``."""
 
-    code = _check_layer(layer)
     act = _ACT_DTYPES.get(dtype)
+    if act is not None:
+        done = (_fast or _ops()).kv8_read_blocks(*layer, block_ids, dtype is torch.bfloat16)
+        if done is not None:
+            if type(done) is int:
+                _native.check(done, "lvb_kv8_read_blocks")
+            return done
+    code = _check_layer(layer)
     if act is None:
         raise KVCacheError("KV8 blocks are read in fp16 or bf16")
     keys = layer.keys
@@ -238,6 +261,11 @@ def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float
     request sees every position up to its own.  ``out`` receives the result
     instead of a new tensor."""
 
+    done = (_fast or _ops()).kv8_attention(query, *layer, *step, scale, out)
+    if done is not None:
+        if type(done) is int:
+            _native.check(done, "lvb_kv8_attention")
+        return done
     code = _check_layer(layer)
     keys = layer.keys
     num_blocks, hkv, block, d = keys.shape

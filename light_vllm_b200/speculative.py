@@ -17,7 +17,8 @@ from torch import Tensor
 from light_vllm_b200 import _native
 from light_vllm_b200.kv8 import _on, _Workspaces
 
-_workspaces = _Workspaces()
+_workspaces = _Workspaces(1)
+_fast = None  # _torch_ops, loaded by the first call
 
 
 def verify_drafts(target_probs: Tensor, draft_tokens: Tensor, accept_uniform: Tensor, sample_uniform: Tensor,
@@ -35,6 +36,16 @@ def verify_drafts(target_probs: Tensor, draft_tokens: Tensor, accept_uniform: Te
     ``draft_probs`` the drafts were looked up rather than drawn, and draft x is
     accepted with probability p(x).  ``max_query_len`` is the longest request's
     row count."""
+
+    global _fast
+    if _fast is None:
+        _fast = _native.torch_ops()
+    done = _fast.verify_drafts(target_probs, draft_tokens, accept_uniform, sample_uniform, query_start, max_query_len,
+                               draft_probs)
+    if done is not None:
+        if type(done) is int:
+            _native.check(done, "lvb_verify_drafts")
+        return done
 
     if target_probs.dtype != torch.float32 or target_probs.dim() != 2:
         raise ValueError("target probabilities must be float32 [rows, vocabulary]")
