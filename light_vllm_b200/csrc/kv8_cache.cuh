@@ -90,7 +90,9 @@ struct AppendArgs {
   int table_rows, hq;
   uint8_t *key_codes, *value_codes;
   float *key_scales, *value_scales;
-  int units;  // blocks to look at (bound)
+  int units;      // blocks to look at (bound)
+  int unit_ctas;  // CTAs that look at them
+  bool query_vec, query_out_vec, key_vec, value_vec, table_vec;  // rows allow 16-byte accesses
 };
 
 // First unit of request r: a request of n tokens touches at most
@@ -105,73 +107,131 @@ __host__ __device__ __forceinline__ int64_t append_units(int64_t num_seqs, int64
   return max_query_len <= 1 ? num_seqs : num_tokens / bs + 2 * num_seqs;
 }
 
-// The elements of a head that lane l holds, kPairs (D / 64) at each of l *
-// kPairs and D / 2 + l * kPairs: a rotation's two halves sit in one lane.
-template <bool kBf16, int D>
-__device__ __forceinline__ void load_row(const uint16_t *row, int lane, float (&x)[D / 32]) {
-  constexpr int kPairs = D / 64;
+// A thread holds pieces of 8 elements of a head: element c * 8 + i of the first
+// half in x[0..7] and of the second in x[8..15], so that a rotation's two sides
+// sit together.  `vec`: rows allow 16-byte loads.
+template <bool kBf16>
+__device__ __forceinline__ void load_piece(const uint16_t *src, bool vec, float *x) {
+  if (vec) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(src);
+    const uint16_t *e = reinterpret_cast<const uint16_t *>(&v);
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    x[i] = to_float<kBf16>(row[lane * kPairs + i]);
-    x[kPairs + i] = to_float<kBf16>(row[D / 2 + lane * kPairs + i]);
+    for (int i = 0; i < 8; ++i) x[i] = to_float<kBf16>(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<kBf16>(src[i]);
   }
 }
 
-template <bool kBf16, int D>
-__device__ __forceinline__ void rotate_row(float (&x)[D / 32], const uint16_t *cos, const uint16_t *sin, int lane) {
-  constexpr int kPairs = D / 64;
+template <bool kBf16>
+__device__ __forceinline__ void store_piece(uint16_t *dst, bool vec, const float *x) {
+  if (vec) {
+    *reinterpret_cast<uint4 *>(dst) =
+        make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]), pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
+  } else {
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const int a = lane * kPairs + i, b = D / 2 + a;
-    const float x1 = x[i], x2 = x[kPairs + i];
-    x[i] = rope_rotate(x1, to_float<kBf16>(cos[a]), -x2, to_float<kBf16>(sin[a]));
-    x[kPairs + i] = rope_rotate(x2, to_float<kBf16>(cos[b]), x1, to_float<kBf16>(sin[b]));
+    for (int i = 0; i < 8; ++i) dst[i] = from_float<kBf16>(x[i]);
   }
+}
+
+// cos and sin of a piece, as raw halves of the tables' rows.
+struct Turn {
+  uint4 c1, c2, s1, s2;
+};
+
+template <int D>
+__device__ __forceinline__ Turn load_turn(const AppendArgs &a, int pos, int c) {
+  const uint16_t *cos = a.cos + static_cast<int64_t>(pos) * D + c * 8, *sin = a.sin + static_cast<int64_t>(pos) * D + c * 8;
+  Turn t;
+  if (a.table_vec) {
+    t.c1 = __ldg(reinterpret_cast<const uint4 *>(cos));
+    t.c2 = __ldg(reinterpret_cast<const uint4 *>(cos + D / 2));
+    t.s1 = __ldg(reinterpret_cast<const uint4 *>(sin));
+    t.s2 = __ldg(reinterpret_cast<const uint4 *>(sin + D / 2));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      reinterpret_cast<uint16_t *>(&t.c1)[i] = cos[i];
+      reinterpret_cast<uint16_t *>(&t.c2)[i] = cos[D / 2 + i];
+      reinterpret_cast<uint16_t *>(&t.s1)[i] = sin[i];
+      reinterpret_cast<uint16_t *>(&t.s2)[i] = sin[D / 2 + i];
+    }
+  }
+  return t;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void rotate(float (&x)[16], const Turn &t) {
+  const uint16_t *c1 = reinterpret_cast<const uint16_t *>(&t.c1), *c2 = reinterpret_cast<const uint16_t *>(&t.c2);
+  const uint16_t *s1 = reinterpret_cast<const uint16_t *>(&t.s1), *s2 = reinterpret_cast<const uint16_t *>(&t.s2);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x[i], b = x[8 + i];
+    x[i] = rope_rotate(a, to_float<kBf16>(c1[i]), -b, to_float<kBf16>(s1[i]));
+    x[8 + i] = rope_rotate(b, to_float<kBf16>(c2[i]), a, to_float<kBf16>(s2[i]));
+  }
+}
+
+template <bool kFp8>
+__device__ __forceinline__ uint2 encode_piece(const float *x, float inv) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    w[i >> 2] |= static_cast<uint32_t>(Code<kFp8>::encode(__fmul_rn(x[i], inv))) << (8 * (i & 3));
+  return make_uint2(w[0], w[1]);
 }
 
 constexpr int kAppendThreads = 128;
 
-// Blocks [0, units) of the grid: one warp for each (unit, KV head, keys or
-// values).  Then one warp for each query row.
+// CTAs [0, unit_ctas) of the grid: one warp for each (unit, KV head, keys or
+// values), four (D = 64: eight) tokens of the block at a time, D / 16 lanes for
+// each, all of a block's 16 tokens in registers between its largest magnitude
+// and its codes (larger blocks are read twice, the second time from the caches).
+// Then one CTA for each token's query heads; its rotation is read once.  Bound
+// by the bytes of the rows: every access is 16 (codes: 8) bytes a lane.
 template <bool kBf16, bool kFp8, int D>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
-  constexpr int kPairs = D / 64;
   using C = Code<kFp8>;
+  constexpr int kLanes = D / 16;  // lanes of a row
   const Step &s = a.step;
-  const int lane = threadIdx.x & 31;
-  const int warps = kAppendThreads / 32;
-  const int warp = threadIdx.x >> 5;
-  const int per_unit = 2 * s.hkv;
-  if (static_cast<int>(blockIdx.x) >= a.units) {  // queries
-    const int rows = s.num_tokens * a.hq;
-    for (int i = (blockIdx.x - a.units) * warps + warp; i < rows; i += (gridDim.x - a.units) * warps) {
-      const int t = i / a.hq, h = i - t * a.hq;
-      const int pos = a.positions[t];
-      if (pos < 0 || pos >= a.table_rows) {
-        record_device_error(LVB_DEVERR_INDEX);
-        continue;
-      }
-      float x[D / 32];
-      load_row<kBf16, D>(a.query + t * a.query_stride + h * D, lane, x);
-      rotate_row<kBf16, D>(x, a.cos + static_cast<int64_t>(pos) * D, a.sin + static_cast<int64_t>(pos) * D, lane);
-      uint16_t *out = a.query_out + t * a.query_out_stride + h * D;
-#pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        out[lane * kPairs + k] = from_float<kBf16>(x[k]);
-        out[D / 2 + lane * kPairs + k] = from_float<kBf16>(x[kPairs + k]);
-      }
+  if (static_cast<int>(blockIdx.x) >= a.unit_ctas) {  // queries
+    const int t = blockIdx.x - a.unit_ctas;
+    const int c = threadIdx.x % kLanes;
+    const int pos = a.positions[t];
+    if (pos < 0 || pos >= a.table_rows) {
+      if (threadIdx.x == 0) record_device_error(LVB_DEVERR_INDEX);
+      return;
+    }
+    const Turn turn = load_turn<D>(a, pos, c);
+#pragma unroll 2
+    for (int h = threadIdx.x / kLanes; h < a.hq; h += kAppendThreads / kLanes) {
+      const uint16_t *src = a.query + t * a.query_stride + h * D + c * 8;
+      float x[16];
+      load_piece<kBf16>(src, a.query_vec, x);
+      load_piece<kBf16>(src + D / 2, a.query_vec, x + 8);
+      rotate<kBf16>(x, turn);
+      uint16_t *dst = a.query_out + t * a.query_out_stride + h * D + c * 8;
+      store_piece<kBf16>(dst, a.query_out_vec, x);
+      store_piece<kBf16>(dst + D / 2, a.query_out_vec, x + 8);
     }
     return;
   }
+  const int per_unit = 2 * s.hkv;
+  const int lane = threadIdx.x & 31;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const int unit = static_cast<int>(task / per_unit), j = static_cast<int>(task - static_cast<int64_t>(unit) * per_unit);
+  if (unit >= a.units) return;
   // The unit's request: the last whose first unit is not past it.
-  const int unit = blockIdx.x;
-  int lo = 0, hi = s.num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first_unit(s, mid) <= unit) lo = mid; else hi = mid - 1;
+  int r = unit;
+  if (s.max_query_len > 1) {
+    int lo = 0, hi = s.num_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first_unit(s, mid) <= unit) lo = mid; else hi = mid - 1;
+    }
+    r = lo;
   }
-  const int r = lo;
   int q0, qlen, computed;
   if (!request_range(s, r, q0, qlen, computed) || qlen == 0) return;
   const int blk = computed / s.bs + unit - first_unit(s, r);
@@ -183,56 +243,85 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     return;
   }
   const int old = first - blk * s.bs;  // earlier tokens in the block
-  for (int j = warp; j < per_unit; j += warps) {
-    const int h = j >> 1;
-    const bool is_key = (j & 1) == 0;
-    const uint16_t *src = is_key ? a.key : a.value;
-    const int64_t stride = is_key ? a.key_stride : a.value_stride;
-    const bool turn = is_key && a.positions != nullptr;
-    auto row = [&](int p, float (&x)[D / 32]) {  // position p's row; false where its rotation is outside the tables
-      const int t = q0 + p - computed;
-      load_row<kBf16, D>(src + t * stride + h * D, lane, x);
-      if (!turn) return true;
-      const int pos = a.positions[t];
-      if (pos < 0 || pos >= a.table_rows) {
+  const int h = j >> 1;
+  const bool is_key = (j & 1) == 0;
+  const uint16_t *src = is_key ? a.key : a.value;
+  const int64_t stride = is_key ? a.key_stride : a.value_stride;
+  const bool turn = is_key && a.positions != nullptr, vec = is_key ? a.key_vec : a.value_vec;
+  constexpr int kTokens = 32 / kLanes, kPasses = 16 / kTokens;
+  const int c = lane % kLanes, sub = lane / kLanes;
+  float x[kPasses][16];
+  uint32_t live = 0;  // bit i: this lane's token of pass i exists
+  float top = 0.f;
+  auto load = [&](int base) {
+    live = 0;
+    int pos[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int p = base + i * kTokens + sub;
+      pos[i] = 0;
+      if (p < end) {
+        live |= 1u << i;
+        if (turn) pos[i] = a.positions[q0 + p - computed];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      if (pos[i] < 0 || (turn && pos[i] >= a.table_rows)) {
         record_device_error(LVB_DEVERR_INDEX);
-        return false;
+        live &= ~(1u << i);
       }
-      rotate_row<kBf16, D>(x, a.cos + static_cast<int64_t>(pos) * D, a.sin + static_cast<int64_t>(pos) * D, lane);
-      return true;
-    };
-    float x[D / 32];
-    float top = 0.f;
-    for (int p = first; p < end; ++p) {
-      if (!row(p, x)) continue;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(x[i]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int64_t at = static_cast<int64_t>(phys) * s.hkv + h;
-    uint8_t *codes = (is_key ? a.key_codes : a.value_codes) + at * s.bs * D;
-    float *scale_at = (is_key ? a.key_scales : a.value_scales) + at;
-    const float s0 = old > 0 ? *scale_at : 0.f;
-    float s1 = fmaxf(s0, __fmul_rn(fminf(top, 3.0e38f), C::kInvTop));
-    if (s1 < kTinyScale) s1 = 0.f;
-    const float inv = s1 > 0.f ? __frcp_rn(s1) : 0.f;
-    if (s1 > s0) {
-      const float ratio = __fmul_rn(s0, inv);
-      for (int i = lane; i < old * D; i += 32) codes[i] = C::encode(__fmul_rn(C::decode(codes[i]), ratio));
-    }
-    for (int p = first; p < end; ++p) {
-      if (!row(p, x)) continue;
-      uint8_t *out = codes + (p - blk * s.bs) * D;
-#pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
-        out[lane * kPairs + k] = C::encode(__fmul_rn(x[k], inv));
-        out[D / 2 + lane * kPairs + k] = C::encode(__fmul_rn(x[kPairs + k], inv));
+      if (live >> i & 1u) {
+        const uint16_t *row = src + (q0 + base + i * kTokens + sub - computed) * stride + h * D + c * 8;
+        load_piece<kBf16>(row, vec, x[i]);
+        load_piece<kBf16>(row + D / 2, vec, x[i] + 8);
       }
     }
-    __syncwarp();  // every lane has read the scale
-    if (lane == 0) *scale_at = s1;
+    if (turn) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+        if (live >> i & 1u) rotate<kBf16>(x[i], load_turn<D>(a, pos[i], c));
+    }
+  };
+  const int64_t at = static_cast<int64_t>(phys) * s.hkv + h;
+  uint8_t *codes = (is_key ? a.key_codes : a.value_codes) + at * s.bs * D;
+  float *scale_at = (is_key ? a.key_scales : a.value_scales) + at;
+  const float s0 = old > 0 ? *scale_at : 0.f;
+  for (int base = first; base < end; base += 16) {
+    load(base);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      if (live >> i & 1u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[i][e]));
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float s1 = fmaxf(s0, __fmul_rn(fminf(top, 3.0e38f), C::kInvTop));
+  if (s1 < kTinyScale) s1 = 0.f;
+  const float inv = s1 > 0.f ? __frcp_rn(s1) : 0.f;
+  if (s1 > s0) {  // earlier tokens' codes, rounded anew
+    const float ratio = __fmul_rn(s0, inv);
+    for (int i = lane; i < old * (D / 16); i += 32) {
+      uint4 v = reinterpret_cast<uint4 *>(codes)[i];
+      uint8_t *e = reinterpret_cast<uint8_t *>(&v);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) e[k] = C::encode(__fmul_rn(C::decode(e[k]), ratio));
+      reinterpret_cast<uint4 *>(codes)[i] = v;
+    }
+  }
+  for (int base = first; base < end; base += 16) {
+    if (end - first > 16) load(base);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      if (live >> i & 1u) {
+        uint8_t *dst = codes + (base + i * kTokens + sub - blk * s.bs) * D + c * 8;
+        *reinterpret_cast<uint2 *>(dst) = encode_piece<kFp8>(x[i], inv);
+        *reinterpret_cast<uint2 *>(dst + D / 2) = encode_piece<kFp8>(x[i] + 8, inv);
+      }
+  }
+  __syncwarp();  // every lane has read the scale
+  if (lane == 0) *scale_at = s1;
 }
 
 // Values of whole blocks in the model's type: out[i][h][slot][d] = code *

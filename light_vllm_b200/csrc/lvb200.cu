@@ -2178,9 +2178,17 @@ int lvb_kv8_append(const uint16_t *query, int64_t query_token_stride, uint16_t *
   a.key_scales = key_scales;
   a.value_scales = value_scales;
   a.units = static_cast<int>(lvb::kv8::append_units(num_seqs, num_tokens, max_query_len, block_size));
-  constexpr int kWarps = lvb::kv8::kAppendThreads / 32;
-  const int64_t query_ctas = query != nullptr ? (num_query_heads * num_tokens + kWarps - 1) / kWarps : 0;
-  const dim3 grid(static_cast<unsigned>(a.units + std::min<int64_t>(query_ctas, 1 << 20)));
+  a.query_vec = aligned16(query) && query_token_stride % 8 == 0;
+  a.query_out_vec = aligned16(query_out) && query_out_stride % 8 == 0;
+  a.key_vec = aligned16(key) && key_token_stride % 8 == 0;
+  a.value_vec = aligned16(value) && value_token_stride % 8 == 0;
+  a.table_vec = aligned16(cos_table) && aligned16(sin_table);
+  constexpr int64_t kWarps = lvb::kv8::kAppendThreads / 32;
+  const int64_t unit_ctas = (a.units * 2 * num_kv_heads + kWarps - 1) / kWarps;
+  const int64_t ctas = unit_ctas + (query != nullptr ? num_tokens : 0);
+  if (ctas > INT_MAX) return fail(LVB_ERR_UNSUPPORTED, "kv8_append: too many tokens in one call");
+  a.unit_ctas = static_cast<int>(unit_ctas);
+  const dim3 grid(static_cast<unsigned>(ctas));
   cudaError_t e = kv8_dispatch(dtype, code_type, head_size, [&](auto b16, auto fp8, auto d) {
     return launch_pdl(lvb::kv8::append_kernel<decltype(b16)::value, decltype(fp8)::value, decltype(d)::value>, grid,
                       dim3(lvb::kv8::kAppendThreads), 0, reinterpret_cast<cudaStream_t>(stream), a);
@@ -2404,8 +2412,9 @@ int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const fl
                    (!draft_probs || (draft_stride % 4 == 0 && aligned16(draft_probs)));
   int64_t chunks = std::max<int64_t>(1, 8LL * sm_count(dev) / num_seqs);
   chunks = std::min<int64_t>({chunks, (vocab_size + 2047) / 2048, lvb::spec::kMaxChunks});
-  const int64_t chunk = ((vocab_size + chunks - 1) / chunks + 3) / 4 * 4;
-  a.chunk = static_cast<int>(chunk);
+  const int64_t segment = ((vocab_size + chunks * lvb::spec::kWarps - 1) / (chunks * lvb::spec::kWarps) + 3) / 4 * 4;
+  a.segment = static_cast<int>(segment);
+  const int64_t chunk = segment * lvb::spec::kWarps;
   const dim3 grid(static_cast<unsigned>((vocab_size + chunk - 1) / chunk), static_cast<unsigned>(num_seqs));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = vec ? launch_pdl(lvb::spec::verify_kernel<true>, grid, dim3(lvb::spec::kVerifyThreads), 0, st, a)

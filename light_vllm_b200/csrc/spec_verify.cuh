@@ -32,7 +32,7 @@ struct VerifyArgs {
   const int32_t *qsl;
   int64_t *out;  // [num_seqs][width]
   int32_t *accepted;
-  int num_seqs, num_rows, width, vocab, chunk;
+  int num_seqs, num_rows, width, vocab, segment;
   unsigned long long *scratch;
 };
 
@@ -41,25 +41,26 @@ __device__ __forceinline__ long long fixed_weight(float w) {
   return __float2ll_rn(w * 0x1p40f);
 }
 
-// Scratch of a request: a counter of its finished CTAs (zero between calls),
-// then the sums of its chunks.  The stride is fixed, so that one request's
-// counter never lies where another call's sums do.
+// The vocabulary is cut into segments, one for each warp; a CTA of kWarps warps
+// takes as many neighbouring ones.  Scratch of a request: a counter of its
+// finished CTAs (zero between calls), then the segments' sums.  The stride is
+// fixed, so that one request's counter never lies where another call's sums do.
+constexpr int kWarps = 8;
+constexpr int kVerifyThreads = kWarps * 32;
 constexpr int kMaxChunks = 126;
-constexpr int kScratchWords = kMaxChunks + 2;  // of 8 bytes
-constexpr int kVerifyThreads = 256;
+constexpr int kScratchWords = kMaxChunks * kWarps + 2;  // of 8 bytes
 
 // One CTA for each (chunk of the vocabulary, request).  Every CTA of a request
 // finds the refused draft for itself (a few loads, in L2 after the first), sums
-// its chunk's weights, and the last one to finish finds the chunk and then the
-// token at which the prefix sum passes the bar.  Bound by reading one row (two
+// its segments' weights, and the last one to finish finds the segment and then
+// the token at which the prefix sum passes the bar.  Bound by reading one row (two
 // after a refusal) of the vocabulary once; a call of one request by the latency
 // of its dependent loads.  kVec: rows allow 16-byte loads.
 template <bool kVec>
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_wait();
-  __shared__ int stop_sm, last_sm, found_sm;
-  __shared__ long long sums[kVerifyThreads / 32];
-  constexpr int kWarps = kVerifyThreads / 32;
+  __shared__ int stop_sm, last_sm, found_sm, segment_sm;
+  __shared__ long long sums[kWarps], before_sm;
   const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = a.qsl[b], rows = a.qsl[b + 1] - row0;
   const int n = rows - 1, first = row0 - b;
@@ -126,10 +127,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       w[i] = residual && v + i == gone ? 0ll : fixed_weight(x[i]);
     }
   };
-  auto range_sum = [&](int v0, int v1, bool residual) {
+  // Sum over [v0, v1) by one warp (every lane's result).
+  auto warp_sum_of = [&](int v0, int v1, bool residual) {
     long long own = 0;
 #pragma unroll 4
-    for (int v = v0 + tid * kStep; v < v1; v += kVerifyThreads * kStep) {
+    for (int v = v0 + lane * kStep; v < v1; v += 32 * kStep) {
       long long w[kStep];
       weights(v, residual, w);
 #pragma unroll
@@ -137,89 +139,96 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
-    __syncthreads();
-    if (lane == 0) sums[warp] = own;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += sums[w];
-    return total;
+    return own;
   };
-  auto bar_of = [&](long long total) {
-    const long long bar = static_cast<long long>(floor(static_cast<double>(a.sample[b]) * static_cast<double>(total)));
-    return max(0ll, min(bar, total - 1));
+  // Inclusive prefix of `own` over the CTA; `all` is the total.
+  auto block_prefix = [&](long long own, long long &all) {
+    long long upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) upto += sums[w];
+      all += sums[w];
+    }
+    return upto;
   };
 
-  const int v0 = min(a.vocab, chunk * a.chunk), v1 = min(a.vocab, v0 + a.chunk);
-  const long long mine = range_sum(v0, v1, true);
+  const int segments = gridDim.x * kWarps;
   unsigned long long *scratch = a.scratch + static_cast<int64_t>(b) * kScratchWords;
-  if (gridDim.x > 1) {
-    if (tid == 0) {
-      scratch[1 + chunk] = static_cast<unsigned long long>(mine);
-      __threadfence();
-      last_sm = atomicAdd(scratch, 1ull) == gridDim.x - 1;
-    }
-    __syncthreads();
-    if (!last_sm) return;
-    __threadfence();
+  const int v0 = min(a.vocab, (chunk * kWarps + warp) * a.segment), v1 = min(a.vocab, v0 + a.segment);
+  const long long mine = warp_sum_of(v0, v1, true);
+  if (lane == 0) __stcg(scratch + 1 + chunk * kWarps + warp, static_cast<unsigned long long>(mine));
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last_sm = gridDim.x == 1 || atomicAdd(scratch, 1ull) == gridDim.x - 1;
+  __syncthreads();
+  if (!last_sm) return;
+  __threadfence();
+  // The segment that the bar falls into, and the prefix sum before it.
+  constexpr int kPer = (kMaxChunks * kWarps + kVerifyThreads - 1) / kVerifyThreads;
+  long long part[kPer], own = 0, total, bar = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = tid * kPer + i;
+    part[i] = at < segments ? static_cast<long long>(__ldcg(scratch + 1 + at)) : 0;
+    own += part[i];
   }
-  // The chunk that the bar falls into, and the prefix sum before it.
-  long long total = 0, before = 0, bar = 0;
-  int at = 0;
-  bool residual = true;
   if (tid == 0) found_sm = a.vocab - 1;
-  if (gridDim.x == 1) {
-    total = mine;
-    bar = bar_of(total);
-  } else {
-    for (int c = 0; c < static_cast<int>(gridDim.x); ++c) total += static_cast<long long>(__ldcg(scratch + 1 + c));
-    bar = bar_of(total);
-    while (at + 1 < static_cast<int>(gridDim.x)) {
-      const long long w = static_cast<long long>(__ldcg(scratch + 1 + at));
-      if (before + w > bar) break;
-      before += w;
-      ++at;
-    }
-    __syncthreads();
-    if (tid == 0) scratch[0] = 0;
-  }
-  int lo = at * a.chunk, hi = min(a.vocab, lo + a.chunk);
-  if (total == 0) {  // nothing is left of p: its own weights, over the whole row
+  bool residual = true;
+  long long upto = block_prefix(own, total) - own;
+  if (tid == 0 && gridDim.x > 1) scratch[0] = 0;
+  if (total == 0) {  // nothing is left of p: its own weights
     residual = false;
-    total = range_sum(0, a.vocab, false);
-    bar = bar_of(total);
-    before = 0;
-    lo = 0;
-    hi = a.vocab;
+    own = 0;
+    for (int i = warp; i < segments; i += kWarps) {
+      const long long w = warp_sum_of(min(a.vocab, i * a.segment), min(a.vocab, (i + 1) * a.segment), false);
+      if (lane == 0) __stcg(scratch + 1 + i, static_cast<unsigned long long>(w));
+    }
+    __threadfence();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = tid * kPer + i;
+      part[i] = at < segments ? static_cast<long long>(__ldcg(scratch + 1 + at)) : 0;
+      own += part[i];
+    }
+    upto = block_prefix(own, total) - own;
   }
   if (total > 0) {
+    bar = static_cast<long long>(floor(static_cast<double>(a.sample[b]) * static_cast<double>(total)));
+    bar = max(0ll, min(bar, total - 1));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (upto <= bar && bar < upto + part[i]) {
+        segment_sm = tid * kPer + i;
+        before_sm = upto;
+      }
+      upto += part[i];
+    }
+    __syncthreads();
+    long long before = before_sm;
+    const int lo = segment_sm * a.segment, hi = min(a.vocab, lo + a.segment);
     for (int v = lo; v < hi; v += kVerifyThreads * kStep) {
       const int own_v = v + tid * kStep;
-      long long w[kStep];
+      long long w[kStep], all;
 #pragma unroll
       for (int i = 0; i < kStep; ++i) w[i] = 0;
       if (own_v < hi) weights(own_v, residual, w);
-      long long own = 0;
+      own = 0;
 #pragma unroll
       for (int i = 0; i < kStep; ++i) own += w[i];
-      long long upto = own;  // inclusive prefix over the CTA
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-      }
-      __syncthreads();
-      if (lane == 31) sums[warp] = upto;
-      __syncthreads();
-      long long all = 0;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        if (k < warp) upto += sums[k];
-        all += sums[k];
-      }
+      const long long mine_upto = block_prefix(own, all);
       if (before + all > bar) {  // the token is here
-        long long sum = before + upto - own;
-        if (sum <= bar && bar < before + upto) {
+        long long sum = before + mine_upto - own;
+        if (sum <= bar && bar < before + mine_upto) {
           int i = 0;
           for (; i < kStep - 1; ++i) {
             sum += w[i];
