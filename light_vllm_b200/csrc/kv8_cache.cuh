@@ -51,6 +51,32 @@ struct Code {
   }
 };
 
+// Two fp16 values of bytes 0, 1 (kHi: 2, 3) of four codes.
+template <bool kFp8>
+struct Pair;
+
+template <>
+struct Pair<false> {
+  static __device__ __forceinline__ uint32_t bias(uint32_t four) { return four ^ 0x80808080u; }
+  template <bool kHi>
+  static __device__ __forceinline__ uint32_t get(uint32_t biased) {
+    const uint32_t v = __byte_perm(biased, 0x64646464u, kHi ? 0x4342 : 0x4140);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+
+template <>
+struct Pair<true> {
+  static __device__ __forceinline__ uint32_t bias(uint32_t four) { return four; }
+  template <bool kHi>
+  static __device__ __forceinline__ uint32_t get(uint32_t four) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(kHi ? four >> 16 : four & 0xffffu),
+                                                     __NV_E4M3);
+    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  }
+};
+
 // The step's packed requests, and the cache they live in.
 struct Step {
   const int32_t *tables;
@@ -107,20 +133,15 @@ __host__ __device__ __forceinline__ int64_t append_units(int64_t num_seqs, int64
   return max_query_len <= 1 ? num_seqs : num_tokens / bs + 2 * num_seqs;
 }
 
-// A thread holds pieces of 8 elements of a head: element c * 8 + i of the first
-// half in x[0..7] and of the second in x[8..15], so that a rotation's two sides
-// sit together.  `vec`: rows allow 16-byte loads.
-template <bool kBf16>
-__device__ __forceinline__ void load_piece(const uint16_t *src, bool vec, float *x) {
-  if (vec) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(src);
-    const uint16_t *e = reinterpret_cast<const uint16_t *>(&v);
+// A thread holds pieces of 8 elements of a head: elements c * 8 .. + 7 of the
+// first half and of the second, so that a rotation's two sides sit together.
+// `vec`: rows allow 16-byte loads.
+__device__ __forceinline__ uint4 load_piece(const uint16_t *src, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4 *>(src);
+  uint4 v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float<kBf16>(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float<kBf16>(src[i]);
-  }
+  for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t *>(&v)[i] = src[i];
+  return v;
 }
 
 template <bool kBf16>
@@ -134,6 +155,12 @@ __device__ __forceinline__ void store_piece(uint16_t *dst, bool vec, const float
   }
 }
 
+template <bool kBf16>
+__device__ __forceinline__ void expand(const uint4 (&raw)[2], float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = to_float<kBf16>(reinterpret_cast<const uint16_t *>(&raw[i >> 3])[i & 7]);
+}
+
 // cos and sin of a piece, as raw halves of the tables' rows.
 struct Turn {
   uint4 c1, c2, s1, s2;
@@ -142,22 +169,8 @@ struct Turn {
 template <int D>
 __device__ __forceinline__ Turn load_turn(const AppendArgs &a, int pos, int c) {
   const uint16_t *cos = a.cos + static_cast<int64_t>(pos) * D + c * 8, *sin = a.sin + static_cast<int64_t>(pos) * D + c * 8;
-  Turn t;
-  if (a.table_vec) {
-    t.c1 = __ldg(reinterpret_cast<const uint4 *>(cos));
-    t.c2 = __ldg(reinterpret_cast<const uint4 *>(cos + D / 2));
-    t.s1 = __ldg(reinterpret_cast<const uint4 *>(sin));
-    t.s2 = __ldg(reinterpret_cast<const uint4 *>(sin + D / 2));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      reinterpret_cast<uint16_t *>(&t.c1)[i] = cos[i];
-      reinterpret_cast<uint16_t *>(&t.c2)[i] = cos[D / 2 + i];
-      reinterpret_cast<uint16_t *>(&t.s1)[i] = sin[i];
-      reinterpret_cast<uint16_t *>(&t.s2)[i] = sin[D / 2 + i];
-    }
-  }
-  return t;
+  return {load_piece(cos, a.table_vec), load_piece(cos + D / 2, a.table_vec), load_piece(sin, a.table_vec),
+          load_piece(sin + D / 2, a.table_vec)};
 }
 
 template <bool kBf16>
@@ -185,35 +198,47 @@ constexpr int kAppendThreads = 128;
 
 // CTAs [0, unit_ctas) of the grid: one warp for each (unit, KV head, keys or
 // values), four (D = 64: eight) tokens of the block at a time, D / 16 lanes for
-// each, all of a block's 16 tokens in registers between its largest magnitude
-// and its codes (larger blocks are read twice, the second time from the caches).
-// Then one CTA for each token's query heads; its rotation is read once.  Bound
-// by the bytes of the rows: every access is 16 (codes: 8) bytes a lane.
+// each.  A block's 16 tokens stay in registers, as they came, between its largest
+// magnitude and its codes, and are rotated twice (larger blocks are read twice,
+// the second time from the caches).  Then one CTA for each token's query heads;
+// its rotation is read once.  Bound by the bytes of the rows: every access is 16
+// (codes: 8) bytes a lane, and rows are asked for before anything that they do
+// not depend on.
 template <bool kBf16, bool kFp8, int D>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
   using C = Code<kFp8>;
   constexpr int kLanes = D / 16;  // lanes of a row
   const Step &s = a.step;
   if (static_cast<int>(blockIdx.x) >= a.unit_ctas) {  // queries
+    constexpr int kHeads = 4, kSlots = kAppendThreads / kLanes;  // heads in flight for a thread, threads of a piece
     const int t = blockIdx.x - a.unit_ctas;
     const int c = threadIdx.x % kLanes;
     const int pos = a.positions[t];
-    if (pos < 0 || pos >= a.table_rows) {
-      if (threadIdx.x == 0) record_device_error(LVB_DEVERR_INDEX);
-      return;
-    }
-    const Turn turn = load_turn<D>(a, pos, c);
-#pragma unroll 2
-    for (int h = threadIdx.x / kLanes; h < a.hq; h += kAppendThreads / kLanes) {
-      const uint16_t *src = a.query + t * a.query_stride + h * D + c * 8;
-      float x[16];
-      load_piece<kBf16>(src, a.query_vec, x);
-      load_piece<kBf16>(src + D / 2, a.query_vec, x + 8);
-      rotate<kBf16>(x, turn);
-      uint16_t *dst = a.query_out + t * a.query_out_stride + h * D + c * 8;
-      store_piece<kBf16>(dst, a.query_out_vec, x);
-      store_piece<kBf16>(dst + D / 2, a.query_out_vec, x + 8);
+    const uint16_t *src = a.query + t * a.query_stride + c * 8;
+    uint16_t *dst = a.query_out + t * a.query_out_stride + c * 8;
+    for (int base = threadIdx.x / kLanes; base < a.hq; base += kHeads * kSlots) {
+      uint4 raw[kHeads][2];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (base + i * kSlots < a.hq) {
+          raw[i][0] = load_piece(src + (base + i * kSlots) * D, a.query_vec);
+          raw[i][1] = load_piece(src + (base + i * kSlots) * D + D / 2, a.query_vec);
+        }
+      if (pos < 0 || pos >= a.table_rows) {
+        if (threadIdx.x == 0) record_device_error(LVB_DEVERR_INDEX);
+        return;
+      }
+      const Turn turn = load_turn<D>(a, pos, c);
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (base + i * kSlots < a.hq) {
+          float x[16];
+          expand<kBf16>(raw[i], x);
+          rotate<kBf16>(x, turn);
+          store_piece<kBf16>(dst + (base + i * kSlots) * D, a.query_out_vec, x);
+          store_piece<kBf16>(dst + (base + i * kSlots) * D + D / 2, a.query_out_vec, x + 8);
+        }
     }
     return;
   }
@@ -238,10 +263,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const int first = max(computed, blk * s.bs), end = min(computed + qlen, (blk + 1) * s.bs);
   if (first >= end) return;
   const int phys = s.tables[r * s.table_stride + blk];
-  if (phys < 0 || phys >= s.num_blocks) {
-    record_device_error(LVB_DEVERR_INDEX);
-    return;
-  }
   const int old = first - blk * s.bs;  // earlier tokens in the block
   const int h = j >> 1;
   const bool is_key = (j & 1) == 0;
@@ -250,50 +271,55 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const bool turn = is_key && a.positions != nullptr, vec = is_key ? a.key_vec : a.value_vec;
   constexpr int kTokens = 32 / kLanes, kPasses = 16 / kTokens;
   const int c = lane % kLanes, sub = lane / kLanes;
-  float x[kPasses][16];
-  uint32_t live = 0;  // bit i: this lane's token of pass i exists
-  float top = 0.f;
+  uint4 raw[kPasses][2];
+  int pos[kPasses];
+  uint32_t live = 0;  // bit i: this lane's token of pass i counts
   auto load = [&](int base) {
     live = 0;
-    int pos[kPasses];
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int p = base + i * kTokens + sub;
-      pos[i] = 0;
       if (p < end) {
+        const int t = q0 + p - computed;
+        const uint16_t *row = src + t * stride + h * D + c * 8;
+        raw[i][0] = load_piece(row, vec);
+        raw[i][1] = load_piece(row + D / 2, vec);
+        pos[i] = turn ? a.positions[t] : 0;
         live |= 1u << i;
-        if (turn) pos[i] = a.positions[q0 + p - computed];
       }
     }
+    if (!turn) return;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if (pos[i] < 0 || (turn && pos[i] >= a.table_rows)) {
+    for (int i = 0; i < kPasses; ++i)
+      if ((live >> i & 1u) && (pos[i] < 0 || pos[i] >= a.table_rows)) {
         record_device_error(LVB_DEVERR_INDEX);
         live &= ~(1u << i);
       }
-      if (live >> i & 1u) {
-        const uint16_t *row = src + (q0 + base + i * kTokens + sub - computed) * stride + h * D + c * 8;
-        load_piece<kBf16>(row, vec, x[i]);
-        load_piece<kBf16>(row + D / 2, vec, x[i] + 8);
-      }
-    }
-    if (turn) {
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i)
-        if (live >> i & 1u) rotate<kBf16>(x[i], load_turn<D>(a, pos[i], c));
-    }
   };
+  auto row_of = [&](int i, float (&x)[16]) {
+    expand<kBf16>(raw[i], x);
+    if (turn) rotate<kBf16>(x, load_turn<D>(a, pos[i], c));
+  };
+  load(first);
+  if (phys < 0 || phys >= s.num_blocks) {
+    record_device_error(LVB_DEVERR_INDEX);
+    return;
+  }
   const int64_t at = static_cast<int64_t>(phys) * s.hkv + h;
   uint8_t *codes = (is_key ? a.key_codes : a.value_codes) + at * s.bs * D;
   float *scale_at = (is_key ? a.key_scales : a.value_scales) + at;
   const float s0 = old > 0 ? *scale_at : 0.f;
+  float top = 0.f;
   for (int base = first; base < end; base += 16) {
-    load(base);
+    if (base > first) load(base);
 #pragma unroll
     for (int i = 0; i < kPasses; ++i)
-      if (live >> i & 1u)
+      if (live >> i & 1u) {
+        float x[16];
+        row_of(i, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[i][e]));
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+      }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -315,9 +341,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < kPasses; ++i)
       if (live >> i & 1u) {
+        float x[16];
+        row_of(i, x);
         uint8_t *dst = codes + (base + i * kTokens + sub - blk * s.bs) * D + c * 8;
-        *reinterpret_cast<uint2 *>(dst) = encode_piece<kFp8>(x[i], inv);
-        *reinterpret_cast<uint2 *>(dst + D / 2) = encode_piece<kFp8>(x[i] + 8, inv);
+        *reinterpret_cast<uint2 *>(dst) = encode_piece<kFp8>(x, inv);
+        *reinterpret_cast<uint2 *>(dst + D / 2) = encode_piece<kFp8>(x + 8, inv);
       }
   }
   __syncwarp();  // every lane has read the scale
@@ -353,10 +381,16 @@ __global__ void __launch_bounds__(256) read_blocks_kernel(const __grid_constant_
     const int64_t at = static_cast<int64_t>(id) * a.hkv + (head - i * a.hkv);
     const float scale = (is_key ? a.key_scales : a.value_scales)[at];
     const uint4 v = reinterpret_cast<const uint4 *>(is_key ? a.key_codes : a.value_codes)[at * a.chunks_per_head + inside];
-    const uint8_t *e = reinterpret_cast<const uint8_t *>(&v);
+    const uint32_t four[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      out[k] = pack2<kBf16>(__fmul_rn(Code<kFp8>::decode(e[2 * k]), scale), __fmul_rn(Code<kFp8>::decode(e[2 * k + 1]), scale));
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = Pair<kFp8>::bias(four[k]);
+      const uint32_t lo = Pair<kFp8>::template get<false>(w), hi = Pair<kFp8>::template get<true>(w);
+      const float2 a2 = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
+      const float2 b2 = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+      out[2 * k] = pack2<kBf16>(__fmul_rn(a2.x, scale), __fmul_rn(a2.y, scale));
+      out[2 * k + 1] = pack2<kBf16>(__fmul_rn(b2.x, scale), __fmul_rn(b2.y, scale));
+    }
   }
   uint4 *dst = reinterpret_cast<uint4 *>(is_key ? a.key_out : a.value_out) + 2 * c;
   dst[0] = make_uint4(out[0], out[1], out[2], out[3]);

@@ -64,32 +64,6 @@ struct AttnArgs {
   uint32_t *tile_counts;  // [CTAs]
 };
 
-// Two fp16 values of bytes 0, 1 (kHi: 2, 3) of four codes.
-template <bool kFp8>
-struct Pair;
-
-template <>
-struct Pair<false> {
-  static __device__ __forceinline__ uint32_t bias(uint32_t four) { return four ^ 0x80808080u; }
-  template <bool kHi>
-  static __device__ __forceinline__ uint32_t get(uint32_t biased) {
-    const uint32_t v = __byte_perm(biased, 0x64646464u, kHi ? 0x4342 : 0x4140);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-};
-
-template <>
-struct Pair<true> {
-  static __device__ __forceinline__ uint32_t bias(uint32_t four) { return four; }
-  template <bool kHi>
-  static __device__ __forceinline__ uint32_t get(uint32_t four) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(kHi ? four >> 16 : four & 0xffffu),
-                                                     __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-  }
-};
-
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -2406,18 +2406,15 @@ int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const fl
   int dev = 0;
   int rc = current_device(&dev);
   if (rc != LVB_OK) return rc;
-  // About eight CTAs of 256 threads for each SM, and chunks of at least 2048
-  // values (two loads of 16 bytes a thread).
-  const bool vec = vocab_size % 4 == 0 && target_stride % 4 == 0 && aligned16(target_probs) &&
-                   (!draft_probs || (draft_stride % 4 == 0 && aligned16(draft_probs)));
-  int64_t chunks = std::max<int64_t>(1, 8LL * sm_count(dev) / num_seqs);
+  // As many CTAs as run at a time, and chunks of at least 2048 values (two
+  // loads of 16 bytes a thread).
+  int64_t chunks = std::max<int64_t>(1, static_cast<int64_t>(lvb::spec::kCtasPerSm) * sm_count(dev) / num_seqs);
   chunks = std::min<int64_t>({chunks, (vocab_size + 2047) / 2048, lvb::spec::kMaxChunks});
   const int64_t segment = ((vocab_size + chunks * lvb::spec::kWarps - 1) / (chunks * lvb::spec::kWarps) + 3) / 4 * 4;
   a.segment = static_cast<int>(segment);
   const int64_t chunk = segment * lvb::spec::kWarps;
   const dim3 grid(static_cast<unsigned>((vocab_size + chunk - 1) / chunk), static_cast<unsigned>(num_seqs));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = vec ? launch_pdl(lvb::spec::verify_kernel<true>, grid, dim3(lvb::spec::kVerifyThreads), 0, st, a)
-                      : launch_pdl(lvb::spec::verify_kernel<false>, grid, dim3(lvb::spec::kVerifyThreads), 0, st, a);
+  cudaError_t e = launch_pdl(lvb::spec::verify_kernel, grid, dim3(lvb::spec::kVerifyThreads), 0, st, a);
   return e == cudaSuccess ? LVB_OK : cuda_fail(e, "verify_kernel launch");
 }

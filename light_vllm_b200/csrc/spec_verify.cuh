@@ -47,6 +47,7 @@ __device__ __forceinline__ long long fixed_weight(float w) {
 // fixed, so that one request's counter never lies where another call's sums do.
 constexpr int kWarps = 8;
 constexpr int kVerifyThreads = kWarps * 32;
+constexpr int kCtasPerSm = 5;
 constexpr int kMaxChunks = 126;
 constexpr int kScratchWords = kMaxChunks * kWarps + 2;  // of 8 bytes
 
@@ -55,9 +56,8 @@ constexpr int kScratchWords = kMaxChunks * kWarps + 2;  // of 8 bytes
 // its segments' weights, and the last one to finish finds the segment and then
 // the token at which the prefix sum passes the bar.  Bound by reading one row (two
 // after a refusal) of the vocabulary once; a call of one request by the latency
-// of its dependent loads.  kVec: rows allow 16-byte loads.
-template <bool kVec>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
+// of its dependent loads.
+__global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_wait();
   __shared__ int stop_sm, last_sm, found_sm, segment_sm;
   __shared__ long long sums[kWarps], before_sm;
@@ -106,36 +106,44 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   const float *q = j < n && a.draft != nullptr ? a.draft + (first + j) * a.draft_stride : nullptr;
   const int64_t gone = j < n && a.draft == nullptr ? a.tokens[first + j] : -1;
 
-  // Weights of the elements v .. v + 3 (kVec) or v.
-  constexpr int kStep = kVec ? 4 : 1;
-  auto weights = [&](int v, bool residual, long long (&w)[kStep]) {
-    float x[kStep], y[kStep];
-    if constexpr (kVec) {
+  // Groups of four elements that lie on 16 bytes in p: group k is elements 4 k -
+  // shift .. + 3, and those outside [lo, hi) count for nothing.  q is read alike
+  // where it lies the same way.
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 2 & 3);
+  const bool alike = q == nullptr || static_cast<int>(reinterpret_cast<uintptr_t>(q) >> 2 & 3) == shift;
+  auto weights = [&](int v, int lo, int hi, bool residual, long long (&w)[4]) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool less = residual && q != nullptr;
+    if (v >= lo && v + 4 <= hi) {
       const float4 t = __ldg(reinterpret_cast<const float4 *>(p + v));
       x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
-      if (residual && q != nullptr) {
+      if (less && alike) {
         const float4 u = __ldg(reinterpret_cast<const float4 *>(q + v));
         y[0] = u.x, y[1] = u.y, y[2] = u.z, y[3] = u.w;
+      } else if (less) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __ldg(q + v + i);
       }
     } else {
-      x[0] = __ldg(p + v);
-      if (residual && q != nullptr) y[0] = __ldg(q + v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i >= lo && v + i < hi) {
+          x[i] = __ldg(p + v + i);
+          if (less) y[i] = __ldg(q + v + i);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) {
-      if (residual && q != nullptr) x[i] = __fsub_rn(x[i], y[i]);
-      w[i] = residual && v + i == gone ? 0ll : fixed_weight(x[i]);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = residual && v + i == gone ? 0ll : fixed_weight(less ? __fsub_rn(x[i], y[i]) : x[i]);
   };
+  auto group_start = [&](int v) { return (v + shift) / 4 * 4 - shift; };
   // Sum over [v0, v1) by one warp (every lane's result).
   auto warp_sum_of = [&](int v0, int v1, bool residual) {
     long long own = 0;
 #pragma unroll 4
-    for (int v = v0 + lane * kStep; v < v1; v += 32 * kStep) {
-      long long w[kStep];
-      weights(v, residual, w);
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) own += w[i];
+    for (int v = group_start(v0) + lane * 4; v < v1; v += 128) {
+      long long w[4];
+      weights(v, v0, v1, residual, w);
+      own += (w[0] + w[1]) + (w[2] + w[3]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
@@ -216,21 +224,17 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     __syncthreads();
     long long before = before_sm;
     const int lo = segment_sm * a.segment, hi = min(a.vocab, lo + a.segment);
-    for (int v = lo; v < hi; v += kVerifyThreads * kStep) {
-      const int own_v = v + tid * kStep;
-      long long w[kStep], all;
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) w[i] = 0;
-      if (own_v < hi) weights(own_v, residual, w);
-      own = 0;
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) own += w[i];
+    for (int v = group_start(lo); v < hi; v += kVerifyThreads * 4) {
+      const int own_v = v + tid * 4;
+      long long w[4] = {0, 0, 0, 0}, all;
+      if (own_v < hi) weights(own_v, lo, hi, residual, w);
+      own = (w[0] + w[1]) + (w[2] + w[3]);
       const long long mine_upto = block_prefix(own, all);
       if (before + all > bar) {  // the token is here
         long long sum = before + mine_upto - own;
         if (sum <= bar && bar < before + mine_upto) {
           int i = 0;
-          for (; i < kStep - 1; ++i) {
+          for (; i < 3; ++i) {
             sum += w[i];
             if (sum > bar) break;
           }

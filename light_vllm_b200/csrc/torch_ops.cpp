@@ -15,6 +15,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -125,6 +127,13 @@ bool rows(const at::Tensor *t, int64_t tokens, int64_t heads, int64_t d, at::Sca
   return t->stride(2) == 1 && (t->size(1) <= 1 || t->stride(1) == d) && t->stride(0) >= t->size(1) * d;
 }
 
+// A new tensor on the current device, from torch's caching allocator without
+// the dispatcher (about 1 us less than at::empty).
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_generic(size, c10::cuda::CUDACachingAllocator::get(),
+                                              c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
+}
+
 int act_of(const at::Tensor &t) {
   return t.scalar_type() == at::kHalf ? LVB_DTYPE_F16 : t.scalar_type() == at::kBFloat16 ? LVB_DTYPE_BF16 : -1;
 }
@@ -166,7 +175,7 @@ PyObject *attention(PyObject *const *args) {
   Scratch ws;
   if (!scratch(kAttentionScratch, l.device, stream, g_attention_bytes(s.n, hq, l.hkv, l.d, s.max_query, s.max_seq), ws))
     Py_RETURN_NONE;
-  const at::Tensor out = given ? *given : at::empty({tokens, hq, l.d}, q->options());
+  const at::Tensor out = given ? *given : fresh({tokens, hq, l.d}, q->scalar_type());
   const int status = g_attention(
       data<uint16_t>(*q), q->stride(0), data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]),
       data<float>(*l.t[3]), data<uint16_t>(out), out.stride(0), data<int32_t>(*s.tables), s.tables->stride(0),
@@ -213,7 +222,7 @@ PyObject *append(PyObject *const *args) {
     Py_RETURN_NONE;
   }
   at::Tensor out;
-  if (query) out = given ? *given : at::empty({tokens, hq, l.d}, query->options());
+  if (query) out = given ? *given : fresh({tokens, hq, l.d}, type);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(l.device)).stream();
   const int status = g_append(
       query ? data<uint16_t>(*query) : nullptr, query ? query->stride(0) : 0, query ? data<uint16_t>(out) : nullptr,
@@ -238,8 +247,8 @@ PyObject *read_blocks(PyObject *const *args) {
   if (!layer(args, l) || !ids || !i32(*ids, l.device) || ids->dim() != 1 || ids->size(0) == 0) Py_RETURN_NONE;
   const bool bf16 = args[5] == Py_True;
   const int64_t n = ids->size(0);
-  const auto options = l.t[0]->options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
-  const at::Tensor keys = at::empty({n, l.hkv, l.bs, l.d}, options), values = at::empty({n, l.hkv, l.bs, l.d}, options);
+  const at::ScalarType type = bf16 ? at::kBFloat16 : at::kHalf;
+  const at::Tensor keys = fresh({n, l.hkv, l.bs, l.d}, type), values = fresh({n, l.hkv, l.bs, l.d}, type);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(l.device)).stream();
   const int status = g_read(data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]), data<float>(*l.t[3]),
                             data<int32_t>(*ids), n, data<uint16_t>(keys), data<uint16_t>(values), l.hkv, l.d, l.bs,
@@ -276,7 +285,7 @@ PyObject *verify(PyObject *const *args) {
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
   Scratch ws;
   if (!scratch(kVerifyScratch, device, stream, g_verify_bytes(n, vocab), ws)) Py_RETURN_NONE;
-  const at::Tensor out = at::empty({n, width}, tokens->options()), accepted = at::empty({n}, start->options());
+  const at::Tensor out = fresh({n, width}, at::kLong), accepted = fresh({n}, at::kInt);
   const bool use = draft && drafts > 0;
   const int status = g_verify(data<float>(*target), rows > 1 ? target->stride(0) : vocab, use ? data<float>(*draft) : nullptr,
                               use ? (drafts > 1 ? draft->stride(0) : vocab) : 0, data<int64_t>(*tokens),
