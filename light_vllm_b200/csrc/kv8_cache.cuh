@@ -60,9 +60,9 @@ struct Pair<false> {
   static __device__ __forceinline__ uint32_t bias(uint32_t four) { return four ^ 0x80808080u; }
   template <bool kHi>
   static __device__ __forceinline__ uint32_t get(uint32_t biased) {
-    const uint32_t v = __byte_perm(biased, 0x64646464u, kHi ? 0x4342 : 0x4140);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t *>(&h);
+    uint32_t d;  // (1024 + 128 + c) - 1152
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(__byte_perm(biased, 0x64646464u, kHi ? 0x4342 : 0x4140)), "r"(0x64806480u));
+    return d;
   }
 };
 
@@ -71,9 +71,12 @@ struct Pair<true> {
   static __device__ __forceinline__ uint32_t bias(uint32_t four) { return four; }
   template <bool kHi>
   static __device__ __forceinline__ uint32_t get(uint32_t four) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(kHi ? four >> 16 : four & 0xffffu),
-                                                     __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+    uint32_t d;
+    if constexpr (kHi)
+      asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(four));
+    else
+      asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(four));
+    return d;
   }
 };
 

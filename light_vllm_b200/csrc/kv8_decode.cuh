@@ -9,8 +9,8 @@
 //     O = sum_j 2^(x_j - m) value code_j        L = sum_j 2^(x_j - m) / w_b
 // give out = O / L: the value scale rides in the exponent, so the weights that
 // enter the second product lie in (0, 1] whatever the scales are, and no code is
-// ever multiplied by a scale.  They enter it as fp16, times 2^8 (kHead) and up to
-// 2^4 (kLazy) more, so that a weight 2^-22 of the largest still has 11 bits; O, L,
+// ever multiplied by a scale.  They enter it as fp16, times 2^6 (kHead) and up to
+// 2^8 (kLazy) more, so that a weight 2^-20 of the largest still has 11 bits; O, L,
 // m and the scores are fp32.  m moves only when it would grow by more than kLazy:
 // a rescaling of O is rare.
 //
@@ -36,8 +36,8 @@
 namespace lvb {
 namespace kv8 {
 
-constexpr float kHead = 8.f;
-constexpr float kLazy = 4.f;
+constexpr float kHead = 6.f;
+constexpr float kLazy = 8.f;
 constexpr int kPage = 16;     // positions a warp takes at a time
 constexpr int kMaxRows = 16;  // query rows of a decode item
 constexpr int kMinRun = 16;   // pages of a CTA, at least: more CTAs only merge more

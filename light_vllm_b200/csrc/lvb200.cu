@@ -2099,9 +2099,10 @@ int kv8_step(const char *what, lvb::kv8::Step &s, const int32_t *tables, int64_t
   if (hkv <= 0 || hkv > 65535) return fail(LVB_ERR_INVALID, "%s: invalid KV head count %lld", what, (long long)hkv);
   if (d != 64 && d != 128)
     return fail(LVB_ERR_UNSUPPORTED, "%s: head size %lld (64 and 128 are covered)", what, (long long)d);
-  if (num_blocks * hkv > INT_MAX) return fail(LVB_ERR_UNSUPPORTED, "%s: over 2^31 - 1 heads of blocks", what);
   if (bs <= 0 || bs % 16 || bs > 1024)
     return fail(LVB_ERR_UNSUPPORTED, "%s: block size %lld (multiples of 16 up to 1024 are covered)", what, (long long)bs);
+  // (the kernels count 16-token pages of one head in 32 bits)
+  if (num_blocks * hkv > INT_MAX / (bs / 16)) return fail(LVB_ERR_UNSUPPORTED, "%s: over 2^31 - 1 pages", what);
   if (num_seqs > 0 && (!tables || !computed || !qsl)) return fail(LVB_ERR_INVALID, "%s: null pointer argument", what);
   s.tables = tables;
   s.table_stride = table_stride;
