@@ -557,6 +557,7 @@ LVB_API int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, 
  * including token t's own (linear layouts: single tokens, drafted tokens
  * under verification, prompt chunks, any mix), K and V read from the 8-bit
  * cache, which must hold this step's tokens already (lvb_kv8_append).
+ * Query and output rows are 16-byte aligned (token strides multiples of 8).
  * Softmax statistics and sums in fp32.  max_query_len is the longest request
  * of the batch (LVB_DEVERR_INDEX and no output for a longer one); max_seq_len
  * guides how contexts are split and need not be exact.  workspace: the bytes

@@ -1,7 +1,8 @@
 // Attention of few query rows over the 8-bit paged cache: requests whose query
-// tokens times the query heads of one KV head are at most 16 (decode steps, and
-// the verification of a draft or two), so that K and V are read once for all of
-// them.  Bound by those bytes.
+// tokens times the query heads of one KV head are at most 64 (decode steps, and
+// the verification of a few drafts).  Up to 32 rows K and V are read once for all
+// of them, above by two row groups that follow each other (the second time from
+// L2).  Bound by those bytes.
 //
 // Mathematics.  With f_b = scale log2(e) key_scale_b and w_b = value_scale_b of
 // a position's block b, x_j = (q . key code_j) f_b + log2 w_b and a running
@@ -22,12 +23,19 @@
 // both operands agree, so lane (g, t) of the fragment takes 16 consecutive bytes
 // of key rows g and g + 8, and of value rows 2t, 2t + 1, 2t + 8, 2t + 9.  A lane
 // only ever reads what it fetched itself: asynchronous copies bring its pieces
-// of the next two pages into its own slots of shared memory, with no barrier.
+// of the next pages into its own slots of shared memory, with no barrier, keys as
+// soon as the present ones are used, values likewise.  A step takes two pages (one
+// where there are many rows), so that their chains of MMAs and exponentials overlap.
+// Nothing of the page loop waits for a load of its own: block ids are read one
+// page ahead of the copies, scales come with the codes (a register that a branch
+// or a select touches waits for its load there: 1 us of each page), and nothing of
+// it lies in local memory.
 //
-// Split.  The pages of all (request, KV head) items are laid end to end and cut
-// into one equal run for each resident CTA, whatever the contexts' lengths; the
-// warps of a CTA take its pages in turn.  An item that ends in another CTA leaves
-// partial (O, m, L) in the workspace, and the last of its CTAs to finish (a
+// Split.  The pages of all (request, KV head, row group) items are laid end to
+// end, each item preceded by kItemCost pages' worth of what it costs besides, and
+// cut into one equal run for each resident CTA, whatever the contexts' lengths;
+// the warps of a CTA take its pages in turn.  An item that ends in another CTA
+// leaves partial (O, m, L) in the workspace, and the last of its CTAs to finish (a
 // counter for each item) sums them in order, so results do not depend on timing.
 #pragma once
 
@@ -39,8 +47,9 @@ namespace kv8 {
 constexpr float kHead = 6.f;
 constexpr float kLazy = 8.f;
 constexpr int kPage = 16;     // positions a warp takes at a time
-constexpr int kMaxRows = 16;  // query rows of a decode item
+constexpr int kMaxRows = 32;  // query rows of a decode item
 constexpr int kMinRun = 16;   // pages of a CTA, at least: more CTAs only merge more
+constexpr int kItemCost = 8;
 
 struct AttnArgs {
   Step step;
@@ -51,13 +60,12 @@ struct AttnArgs {
   const uint8_t *key_codes, *value_codes;
   const float *key_scales, *value_scales;
   int hq, group;
-  bool query_vec, out_vec;  // rows allow 16-byte loads, 8-byte stores
   float scale_log2;  // softmax scale * log2(e)
   int few_rows;      // requests of up to this many query rows are the decode kernel's
   // Pieces of items that cross CTAs, and how many of an item's CTAs are done
   // (kept at the CTA that the item begins in; zero between calls).
-  float *part_o;         // decode kernel: [2 * CTAs][kMaxRows][D]
-  float2 *part_ml;       // [2 * CTAs][kMaxRows]: m, L
+  float *part_o;         // decode kernel: [2 * CTAs][its rows][D]
+  float2 *part_ml;       // [2 * CTAs][its rows]: m, L
   uint32_t *counts;      // [CTAs]
   float *tile_o;         // tile kernel: [2 * CTAs][kTileRows][D]
   float2 *tile_ml;       // [2 * CTAs][kTileRows]
@@ -92,32 +100,6 @@ __device__ __forceinline__ void lds_8(uint32_t (&v)[2], uint32_t src) {
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) { return pack2<false>(lo, hi); }
 
-// Eight elements of a row, one load where rows are 16-byte aligned.
-template <bool kBf16>
-__device__ __forceinline__ void load8(const uint16_t *src, bool some, bool vec, float (&x)[8]) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  uint16_t *e = reinterpret_cast<uint16_t *>(&v);
-  if (some && vec) {
-    v = *reinterpret_cast<const uint4 *>(src);
-  } else if (some) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = src[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_float<kBf16>(e[i]);
-}
-
-template <bool kBf16>
-__device__ __forceinline__ void store8(uint16_t *dst, bool vec, const float (&x)[8]) {
-  if (vec) {
-    *reinterpret_cast<uint4 *>(dst) =
-        make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]), pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dst[i] = from_float<kBf16>(x[i]);
-  }
-}
-
 // The power of two that brings `top` to [2^to, 2^(to + 1)), within the normal range.
 __device__ __forceinline__ float scale_to(float top, int to) {
   const int field = static_cast<int>(__float_as_uint(top) >> 23);
@@ -126,9 +108,9 @@ __device__ __forceinline__ float scale_to(float top, int to) {
 
 __device__ __forceinline__ void named_barrier_256() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// A row of queries as fp16 times 2^shift (returned as 2^-shift): fp16 rows as
-// they are; bf16 rows with their largest element brought to [2^7, 2^8), which
-// keeps every element down to 2^-22 of it exact, and smaller ones to 2^-32 of it.
+// A row of queries as fp16 times 2^shift (returned): fp16 rows as they are; bf16
+// rows with their largest element brought to [2^7, 2^8), which keeps every element
+// down to 2^-22 of it exact, and smaller ones to 2^-32 of it.
 template <bool kBf16, int N>
 __device__ __forceinline__ float query_shift(const float (&x)[N]) {
   if constexpr (!kBf16) {
@@ -145,9 +127,10 @@ __device__ __forceinline__ float query_shift(const float (&x)[N]) {
 
 // One run of pages of one item.
 struct Segment {
-  int r, kvh, first, last;  // pages [first, last)
-  int pages;                // of the whole item
-  int q0, rows, computed;
+  int r, kvh, group;        // the item
+  int first, last, pages;   // pages [first, last) of it, and all
+  int q0, rows, computed;   // rows: of the whole request and KV head
+  long long at;             // flat place of the item's first page
 };
 
 // kNT: tiles of 8 query rows.
@@ -158,15 +141,69 @@ struct DecodeCfg {
   static constexpr int kCtasPerSm = kNT == 1 ? 2 : 1;
   static constexpr int kRows = 8 * kNT;
   static constexpr int kPad = D + 4;                // floats of a row of O in shared memory
-  static constexpr int kPageBytes = 2 * kPage * D;  // K and V
-  static constexpr int kSlots = 2;                  // pages in flight for each warp
-  static constexpr int kRingBytes = kWarps * kSlots * kPageBytes;
-  static constexpr int kOBytes = kWarps * kRows * kPad * 4;
-  static constexpr int kSmemBytes = kRingBytes + kOBytes;
+  static constexpr int kPages = kNT <= 2 ? 2 : 1;   // pages of a step
+  static constexpr int kSide = kPage * D;           // K (or V) of a page
+  static constexpr int kRingBytes = kWarps * kPages * 2 * kSide;
+  // The warps' sums meet in shared memory kMeet warps at a time.
+  static constexpr int kMeet = kNT <= 1 ? 8 : 4;
+  static constexpr int kOBytes = kMeet * kRows * kPad * 4;
+  static constexpr int kQBytes = kNT == 1 ? 0 : kNT * (D / 16) * 32 * 8;  // query fragments
+  static constexpr int kScaleOff = kRingBytes + kOBytes + kQBytes;  // float [warp][page]{key, value}
+  static constexpr int kSmemBytes = kScaleOff + kWarps * kPages * 8;
 };
 
 __device__ __forceinline__ void cp_async_8(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A request of the decode kernel's: its first token, tokens and computed count;
+// n = 0: not its, or refused.
+struct Request {
+  int q0, n, computed;
+};
+
+__device__ __forceinline__ Request decode_request(const Step &s, int group, int few_rows, int r) {
+  Request q;
+  if (!request_range(s, r, q.q0, q.n, q.computed) || q.n * group > few_rows) q.n = 0;
+  return q;
+}
+
+__device__ __forceinline__ int pages_of(const Request &q) { return (q.computed + q.n + kPage - 1) / kPage; }
+
+// To the run's next item with pages of the run; false at its end.  `left` rows of
+// the flat order are walked in steps of an item's cost, rounded up to `unit`.
+__device__ __noinline__ bool next_item(const Step &s, int group_heads, int few_rows, int rows_each, int unit, long long end,
+                                       Segment &seg) {
+  const int cost = (seg.pages + kItemCost + unit - 1) / unit * unit;
+  const long long at = seg.at + cost;
+  if (at >= end) return false;
+  int r = seg.r, kvh = seg.kvh, group = seg.group + 1;
+  if (group * rows_each >= seg.rows) {
+    group = 0;
+    if (++kvh == s.hkv) {
+      kvh = 0;
+      Request q;
+      do {
+        if (++r == s.num_seqs) return false;
+        q = decode_request(s, group_heads, few_rows, r);
+      } while (q.n == 0);
+      seg.r = r;
+      seg.q0 = q.q0;
+      seg.computed = q.computed;
+      seg.rows = q.n * group_heads;
+      seg.pages = pages_of(q);
+    }
+  }
+  seg.kvh = kvh;
+  seg.group = group;
+  seg.at = at;
+  seg.first = 0;  // (the run began before)
+  seg.last = static_cast<int>(end - at < seg.pages ? end - at : seg.pages);
+  return true;
 }
 
 template <bool kBf16, bool kFp8, int D, int kNT>
@@ -181,202 +218,220 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   constexpr int kVWords = D / 32;   // words of a value row that a lane takes
   constexpr float kNone = -1e30f;   // m before any position
   extern __shared__ __align__(16) uint8_t smem[];
-  float *o_sm = reinterpret_cast<float *>(smem + Cfg::kRingBytes);  // [warp][row][kPad]
+  float *o_sm = reinterpret_cast<float *>(smem + Cfg::kRingBytes);                        // [kMeet][row][kPad]
+  uint2 *q_sm = reinterpret_cast<uint2 *>(smem + Cfg::kRingBytes + Cfg::kOBytes);         // [kNT][kKSteps][32]
   __shared__ float m_sm[kWarps][kRows], l_sm[kWarps][kRows];
-  __shared__ int scan[kWarps];
-  __shared__ long long start_pages;  // pages before the run's first request
-  __shared__ int start_request, last_sm;
+  __shared__ long long scan[kWarps];
+  __shared__ Segment start_sm;
+  __shared__ int last_sm;
   pdl_wait();
   const Step &s = a.step;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
 
-  // Pages of request r's items (0: not this kernel's, or refused).
-  auto request_pages = [&](int r) {
-    int q0, n, c;
-    if (!request_range(s, r, q0, n, c) || n == 0 || n * a.group > a.few_rows) return 0;
-    return (c + n + kPage - 1) / kPage;
+  // What the items of a request come to (rounded up to `unit` each).
+  auto request_cost = [&](const Request &q, int unit) {
+    if (q.n == 0) return 0ll;
+    const int cost = (pages_of(q) + kItemCost + unit - 1) / unit * unit;
+    return static_cast<long long>(cost) * ((q.n * a.group + kRows - 1) / kRows) * s.hkv;
   };
-  // Exclusive prefix of a value over the CTA; `sum` is the total.
-  auto block_scan = [&](int v, int &sum) {
-    int x = v;
+  // Inclusive prefix over the CTA; `all` is the total.
+  auto block_scan = [&](long long v, long long &all) {
+    long long x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) scan[warp] = x;
     __syncthreads();
-    int before = 0;
-    sum = 0;
+    all = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += scan[w];
-      sum += scan[w];
+      if (w < warp) x += scan[w];
+      all += scan[w];
     }
-    return before + x - v;
+    return x;
   };
-
-  // The whole batch's pages, the run of each CTA, and where this one's begins.
-  long long total = 0;
-  int mine = 0, sum = 0, ex = 0;
+  // A batch that gives every CTA at most kSmallRun pages is cut at the items'
+  // starts: a piece each for the CTAs, and short items are not cut at all.
+  // Otherwise the flat order is cut into equal runs.
+  constexpr int kSmallRun = kMinRun + kItemCost;
+  Request mine{};
+  long long total = 0, padded = 0, sum, upto = 0;
+#pragma unroll 1
   for (int base = 0; base < s.num_seqs; base += kThreads) {
-    mine = base + tid < s.num_seqs ? request_pages(base + tid) : 0;
-    ex = block_scan(mine, sum);
-    total += static_cast<long long>(sum) * s.hkv;
+    mine.n = 0;
+    if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
+    upto = block_scan(request_cost(mine, kSmallRun), sum);
+    padded += sum;
+    if (padded > static_cast<long long>(kSmallRun) * gridDim.x) break;
   }
-  long long run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < kMinRun) run = kMinRun;
+  const int unit = padded <= static_cast<long long>(kSmallRun) * gridDim.x ? kSmallRun : 1;
+  if (unit == 1) {
+#pragma unroll 1
+    for (int base = 0; base < s.num_seqs; base += kThreads) {
+      if (s.num_seqs > kThreads) {
+        mine.n = 0;
+        if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
+      }
+      upto = block_scan(request_cost(mine, 1), sum);
+      total += sum;
+    }
+  } else {
+    total = padded;
+  }
+  const long long run = unit > 1 ? unit : (total + gridDim.x - 1) / gridDim.x;
   const long long begin = run * blockIdx.x;
   if (begin >= total) return;
   const long long end = begin + run < total ? begin + run : total;
   {
     long long before = 0;
+#pragma unroll 1
     for (int base = 0; base < s.num_seqs; base += kThreads) {
       if (s.num_seqs > kThreads) {
-        mine = base + tid < s.num_seqs ? request_pages(base + tid) : 0;
-        ex = block_scan(mine, sum);
+        mine.n = 0;
+        if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
+        upto = block_scan(request_cost(mine, unit), sum);
       }
-      const long long lo = before + static_cast<long long>(ex) * s.hkv, hi = lo + static_cast<long long>(mine) * s.hkv;
+      const long long hi = before + upto, lo = hi - request_cost(mine, unit);
       if (lo <= begin && begin < hi) {
-        start_request = base + tid;
-        start_pages = lo;
+        // The run begins in one of this thread's request's items.
+        const int pages = pages_of(mine), cost = (pages + kItemCost + unit - 1) / unit * unit, rows = mine.n * a.group;
+        const int item = static_cast<int>((begin - lo) / cost), groups = (rows + kRows - 1) / kRows;
+        Segment seg;
+        seg.r = base + tid;
+        seg.kvh = item / groups;
+        seg.group = item % groups;
+        seg.at = lo + static_cast<long long>(item) * cost + kItemCost;
+        seg.q0 = mine.q0;
+        seg.rows = rows;
+        seg.computed = mine.computed;
+        seg.pages = pages;
+        seg.first = static_cast<int>(begin > seg.at ? begin - seg.at : 0);
+        seg.last = static_cast<int>(end - seg.at < pages ? (end > seg.at ? end - seg.at : 0) : pages);
+        start_sm = seg;
       }
-      before += static_cast<long long>(sum) * s.hkv;
+      if (s.num_seqs > kThreads) before += sum;
     }
     __syncthreads();
   }
-
-  auto describe = [&](int r, int kvh, int first, int left, Segment &seg) {
-    seg.r = r;
-    seg.kvh = kvh;
-    seg.q0 = s.qsl[r];
-    seg.computed = s.computed[r];
-    const int n = s.qsl[r + 1] - seg.q0;
-    seg.rows = n * a.group;
-    seg.pages = (seg.computed + n + kPage - 1) / kPage;
-    seg.first = first;
-    seg.last = left < seg.pages - first ? first + left : seg.pages;
-  };
-  int left = static_cast<int>(end - begin);  // pages of the run from the present segment on
-  Segment seg;
-  {
-    const int r = start_request;
-    const int pages = request_pages(r);
-    const int inside = static_cast<int>(begin - start_pages);
-    describe(r, inside / pages, inside % pages, left, seg);
-  }
-  // The segment after `from`; false at the end of the run.
-  auto next_segment = [&](const Segment &from, Segment &to) {
-    const int rest = left - (from.last - from.first);
-    if (rest <= 0) return false;
-    int r = from.r, kvh = from.kvh + 1;
-    if (kvh == s.hkv) {
-      kvh = 0;
-      do {
-        ++r;
-      } while (request_pages(r) == 0);  // pages are left, so a request is
-    }
-    describe(r, kvh, 0, rest, to);
-    return true;
-  };
+  // Walked twice, by the page loop and, ahead of it, by the copies.
+  Segment walk_m = start_sm, walk_f = walk_m;
+  auto advance = [&](Segment &walk) { return next_item(s, a.group, a.few_rows, kRows, unit, end, walk); };
 
   // This lane's pieces of a page: 2 kKChunks of 16 bytes of K, four of 4 kVWords bytes of V.
-  const uint32_t ring = smem_u32(smem) + warp * (Cfg::kSlots * Cfg::kPageBytes);
+  constexpr int kPages = Cfg::kPages, kSideBytes = Cfg::kSide;
+  const uint32_t ring = smem_u32(smem) + warp * (kPages * 2 * kSideBytes);  // [page][K, V]
   const int ppb = s.bs / kPage;
-  const uint32_t head_bytes = static_cast<uint32_t>(s.bs) * D;
+  const uint32_t per_block = ppb > 1 ? 0xffffffffu / ppb + 1 : 0u;  // 2^32 / ppb, rounded up: exact for p * ppb < 2^32
+  auto block_of = [&](int p) { return ppb == 1 ? p : static_cast<int>(__umulhi(p, per_block)); };
   const uint8_t *k_lane = a.key_codes + g * D + t * 16;
   const uint8_t *v_lane = a.value_codes + 2 * t * D + g * (D / 8);
-  float ks_ring[Cfg::kSlots], vs_ring[Cfg::kSlots];  // scales; ks NaN: block id out of range
-  auto fetch = [&](const Segment &of, int p, int slot) {
-    const int blk = ppb == 1 ? p : p / ppb;
-    int phys = s.tables[of.r * s.table_stride + blk];
-    const bool bad = static_cast<uint32_t>(phys) >= static_cast<uint32_t>(s.num_blocks);
-    if (bad) {
-      record_device_error(LVB_DEVERR_INDEX);
-      phys = 0;
+  // Scales come the same way: lane 2 i brings page i's key scale, 2 i + 1 its value scale.
+  const uint32_t scale_ring = smem_u32(smem) + Cfg::kScaleOff + warp * (kPages * 8);
+  const float *scale_lane = (lane & 1) == 0 ? a.key_scales : a.value_scales;
+  // The next step's pages (f_p .. of f_last, their KV head and table) and their
+  // blocks, read a step ahead so that no copy waits for them.
+  const int32_t *f_table = s.tables + walk_f.r * s.table_stride;
+  int f_p = walk_f.first + warp * kPages, f_last = walk_f.last, f_kvh = walk_f.kvh, f_phys[kPages];
+  asm volatile("" : "+l"(f_table), "+r"(f_last), "+r"(f_kvh));  // not to be read again from local memory
+  bool f_more = true;
+  uint32_t f_at[kPages];   // the pages' places, in pages of one head, for the values that follow the keys
+  uint32_t f_there = 0;    // bit i: page i of the step that was fetched last exists
+  auto settle = [&]() {
+#pragma unroll 1
+    while (f_more && f_p >= f_last) {
+      f_more = advance(walk_f);
+      f_table = s.tables + walk_f.r * s.table_stride;
+      f_p = walk_f.first + warp * kPages;
+      f_last = walk_f.last;
+      f_kvh = walk_f.kvh;
+      asm volatile("" : "+l"(f_table), "+r"(f_last), "+r"(f_kvh));
     }
-    const uint32_t h = static_cast<uint32_t>(phys) * s.hkv + of.kvh;
-    ks_ring[slot] = bad ? NAN : __ldg(a.key_scales + h);
-    vs_ring[slot] = __ldg(a.value_scales + h);
-    const uint64_t at = static_cast<uint64_t>(h) * head_bytes + (p - blk * ppb) * (kPage * D);
-    const uint8_t *kp = k_lane + at, *vp = v_lane + at;
-    const uint32_t dst = ring + slot * Cfg::kPageBytes;
+    if (f_more) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < kKChunks; ++c)
-        cp_async_16(dst + ((i * kKChunks + c) * 32 + lane) * 16, kp + i * 8 * D + c * 64, 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t *src = vp + ((i & 1) + (i >> 1) * 8) * D;
-      if constexpr (D == 128)
-        cp_async_16(dst + kPage * D + (i * 32 + lane) * 16, src, 16);
-      else
-        cp_async_8(dst + kPage * D + (i * 32 + lane) * 8, src);
+      for (int i = 0; i < kPages; ++i) f_phys[i] = __ldg(f_table + block_of(min(f_p + i, f_last - 1)));
     }
   };
-
-  // Pages of the run that this warp takes, in order, across segments: (fs, fp)
-  // is the next one to fetch.
-  Segment fs = seg;
-  int fp = seg.first + warp;
-  int fleft = left;
-  bool fmore = true;
-  auto fetch_next = [&](int slot) {
-    while (fmore && fp >= fs.last) {
-      Segment n;
-      const int keep = left;
-      left = fleft;
-      fmore = next_segment(fs, n);
-      left = keep;
-      if (fmore) {
-        fleft -= fs.last - fs.first;
-        fs = n;
-        fp = fs.first + warp;
+  auto fetch_keys = [&]() {
+    f_there = 0;
+    if (f_more) {
+#pragma unroll
+      for (int i = 0; i < kPages; ++i) {
+        const bool bad = static_cast<uint32_t>(f_phys[i]) >= static_cast<uint32_t>(s.num_blocks);
+        const uint32_t h = bad ? 0u : static_cast<uint32_t>(f_phys[i]) * s.hkv + f_kvh;
+        f_at[i] = (h - block_of(f_p + i)) * ppb + f_p + i;
+        if (bad && f_p + i < f_last) record_device_error(LVB_DEVERR_INDEX);
+        if (!bad && f_p + i < f_last) {
+          f_there |= 1u << i;
+          if (lane >> 1 == i) cp_async_4(scale_ring + lane * 4, scale_lane + h);
+          const uint8_t *src = k_lane + static_cast<uint64_t>(f_at[i]) * kSideBytes;
+          const uint32_t dst = ring + i * (2 * kSideBytes);
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < kKChunks; ++c)
+              cp_async_16(dst + ((r * kKChunks + c) * 32 + lane) * 16, src + r * 8 * D + c * 64, 16);
+        }
       }
-    }
-    if (fmore) {
-      fetch(fs, fp, slot);
-      fp += kWarps;
     }
     cp_async_commit();
   };
+  auto fetch_values = [&]() {  // of the pages whose keys were fetched, then on to the next step's
 #pragma unroll
-  for (int i = 0; i < Cfg::kSlots; ++i) fetch_next(i);
-  int slot = 0;
+    for (int i = 0; i < kPages; ++i)
+      if (f_there >> i & 1u) {
+        const uint8_t *src = v_lane + static_cast<uint64_t>(f_at[i]) * kSideBytes;
+        const uint32_t dst = ring + i * (2 * kSideBytes) + kSideBytes;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (D == 128)
+            cp_async_16(dst + (r * 32 + lane) * 16, src + ((r & 1) + (r >> 1) * 8) * D, 16);
+          else
+            cp_async_8(dst + (r * 32 + lane) * 8, src + ((r & 1) + (r >> 1) * 8) * D);
+        }
+      }
+    cp_async_commit();
+    f_p += kWarps * kPages;
+    settle();
+  };
+  settle();
+  fetch_keys();
+  uint32_t there = f_there;  // the present step's
+  fetch_values();
 
   bool more = true;
+#pragma unroll 1
   while (more) {
+    const Segment seg = walk_m;  // in registers
+    if (seg.first >= seg.last) {  // nothing of this item but its beginning
+      more = advance(walk_m);
+      continue;
+    }
+    const int row0 = seg.group * kRows, rows = min(seg.rows - row0, kRows);
     // Query rows n = g (B fragments), and rows 2t, 2t + 1 (scores): row i is
     // token i / group, head i % group.
-    uint32_t qb[kNT][kKSteps][2];
+    uint32_t qb[kNT == 1 ? kKSteps : 1][2];
     float f[kNT][2];
     int limit[kNT][2];  // last position that the row sees
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
       const int row = n * 8 + g;
-      const bool ok = row < seg.rows;
-      const int tok = ok ? row / a.group : 0, head = ok ? row - tok * a.group : 0;
+      const bool ok = row < rows;
+      const int tok = ok ? (row0 + row) / a.group : 0, head = ok ? row0 + row - tok * a.group : 0;
       const uint16_t *src = a.query + (seg.q0 + tok) * a.query_stride + (seg.kvh * a.group + head) * D + t * 16;
       float x[kKChunks * 16];
 #pragma unroll
-      for (int c = 0; c < kKChunks; ++c) {
-        if (a.query_vec) {
+      for (int c = 0; c < kKChunks; ++c)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (ok) v = *reinterpret_cast<const uint4 *>(src + c * 64 + i * 8);
-            const uint16_t *e = reinterpret_cast<const uint16_t *>(&v);
+        for (int i = 0; i < 2; ++i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (ok) v = *reinterpret_cast<const uint4 *>(src + c * 64 + i * 8);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[c * 16 + i * 8 + k] = to_float<kBf16>(e[k]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[c * 16 + i] = ok ? to_float<kBf16>(src[c * 64 + i]) : 0.f;
+          for (int k = 0; k < 8; ++k) x[c * 16 + i * 8 + k] = to_float<kBf16>(reinterpret_cast<const uint16_t *>(&v)[k]);
         }
-      }
       const float up = query_shift<kBf16>(x);
       const float fr = a.scale_log2 / up;
       const int lim = ok ? seg.computed + tok : -1;
@@ -387,10 +442,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       }
 #pragma unroll
       for (int k = 0; k < kKSteps; ++k) {
-        qb[n][k][0] = pack_half(x[4 * k] * up, x[4 * k + 1] * up);
-        qb[n][k][1] = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
+        const uint32_t lo = pack_half(x[4 * k] * up, x[4 * k + 1] * up), hi = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
+        if constexpr (kNT == 1) {
+          qb[k][0] = lo, qb[k][1] = hi;
+        } else if (warp == n) {
+          q_sm[(n * kKSteps + k) * 32 + lane] = make_uint2(lo, hi);
+        }
       }
     }
+    if constexpr (kNT > 1) __syncthreads();
     float o[kNT][kDTiles][4], m[kNT][2], l[kNT][2];
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
@@ -402,60 +462,75 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       for (int e = 0; e < 2; ++e) m[n][e] = kNone, l[n][e] = 0.f;
     }
 
-    for (int p = seg.first + warp; p < seg.last; p += kWarps) {
-      cp_async_wait_group<Cfg::kSlots - 1>();
-      const uint32_t src = ring + slot * Cfg::kPageBytes;
-      const float ks = slot == 0 ? ks_ring[0] : ks_ring[1], vs = slot == 0 ? vs_ring[0] : vs_ring[1];
-      const bool bad = ks != ks;
-      uint32_t kreg[2][kKChunks][4], vreg[4][kVWords];
+    int last = seg.last, mask_from = (seg.computed + 1) / kPage;  // pages from there on are not seen whole by every row
+    asm volatile("" : "+r"(last), "+r"(mask_from));               // in registers
+#pragma unroll 1
+    for (int p = seg.first + warp * kPages; p < last; p += kWarps * kPages) {
+      // Scores: positions g and g + 8 by rows 2t and 2t + 1 of each page.
+      cp_async_wait_group<1>();
+      __syncwarp();  // (the scales are other lanes' copies)
+      float sc[kPages][kNT][4], ks[kPages], vs[kPages];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kPages; ++i) {
+        const uint32_t src = ring + i * (2 * kSideBytes);
+        uint32_t scales[2], kreg[2][kKChunks][4];
+        lds_8(scales, scale_ring + i * 8);
+        ks[i] = __uint_as_float(scales[0]), vs[i] = __uint_as_float(scales[1]);
 #pragma unroll
-        for (int c = 0; c < kKChunks; ++c) lds_16(kreg[i][c], src + ((i * kKChunks + c) * 32 + lane) * 16);
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (D == 128)
-          lds_16(vreg[i], src + kPage * D + (i * 32 + lane) * 16);
-        else
-          lds_8(vreg[i], src + kPage * D + (i * 32 + lane) * 8);
-      }
-      // Scores: positions g and g + 8 by rows 2t and 2t + 1.
-      float sc[kNT][4];
+          for (int c = 0; c < kKChunks; ++c) lds_16(kreg[r][c], src + ((r * kKChunks + c) * 32 + lane) * 16);
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        for (int n = 0; n < kNT; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kKSteps; ++k) {
-        const uint32_t w0 = P::bias(kreg[0][k >> 2][k & 3]), w1 = P::bias(kreg[1][k >> 2][k & 3]);
-        const uint32_t ka[4] = {P::template get<false>(w0), P::template get<false>(w1), P::template get<true>(w0),
-                                P::template get<true>(w1)};
+        for (int k = 0; k < kKSteps; ++k) {
+          const uint32_t w0 = P::bias(kreg[0][k >> 2][k & 3]), w1 = P::bias(kreg[1][k >> 2][k & 3]);
+          const uint32_t ka[4] = {P::template get<false>(w0), P::template get<false>(w1), P::template get<true>(w0),
+                                  P::template get<true>(w1)};
+          if constexpr (kNT == 1) {
+            mma_16816_nv<false>(sc[i][0], ka, qb[k][0], qb[k][1]);
+          } else {
 #pragma unroll
-        for (int n = 0; n < kNT; ++n) mma_16816_nv<false>(sc[n], ka, qb[n][k][0], qb[n][k][1]);
-      }
-      const float vw = vs > 0.f ? vs : 1.f;
-      const float lw = log2_fast(vw), iw = rcp_fast(vw);
-      const bool masked = bad || p * kPage + kPage - 1 > seg.computed;
-      // Exponents against the present m, plus kHead.
-      float y[kNT][4];
-      auto exponents = [&]() {
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[n][i] = fmaf(sc[n][i], f[n][i & 1] * ks, lw - m[n][i & 1] + kHead);
-        if (masked) {
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (bad || p * kPage + g + (i >> 1) * 8 > limit[n][i & 1]) y[n][i] = -INFINITY;
+            for (int n = 0; n < kNT; ++n) {
+              const uint2 b = q_sm[(n * kKSteps + k) * 32 + lane];
+              mma_16816_nv<false>(sc[i][n], ka, b.x, b.y);
+            }
+          }
         }
+      }
+      const uint32_t now = there;
+      __syncwarp();
+      fetch_keys();  // the present ones are in registers and used
+      there = f_there;
+      const bool masked = now != (1u << kPages) - 1 || p + kPages - 1 >= mask_from;
+      // Exponents against the present m, plus kHead.
+      float y[kPages][kNT][4], lw[kPages], iw[kPages];
+#pragma unroll
+      for (int i = 0; i < kPages; ++i) {
+        const float vw = (now >> i & 1u) && vs[i] > 0.f ? vs[i] : 1.f;  // (a page that does not exist brings no scales)
+        lw[i] = log2_fast(vw);
+        iw[i] = rcp_fast(vw);
+      }
+      auto exponents = [&]() {
+        float high = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPages; ++i)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) {
+            const float b0 = (lw[i] + kHead) - m[n][0], b1 = (lw[i] + kHead) - m[n][1];
+            const float f0 = f[n][0] * ks[i], f1 = f[n][1] * ks[i];
+            y[i][n][0] = fmaf(sc[i][n][0], f0, b0), y[i][n][1] = fmaf(sc[i][n][1], f1, b1);
+            y[i][n][2] = fmaf(sc[i][n][2], f0, b0), y[i][n][3] = fmaf(sc[i][n][3], f1, b1);
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!(now >> i & 1u) || (p + i) * kPage + g + (e >> 1) * 8 > limit[n][e & 1]) y[i][n][e] = -INFINITY;
+            }
+            high = fmaxf(fmaxf(fmaxf(y[i][n][0], y[i][n][1]), fmaxf(y[i][n][2], y[i][n][3])), high);
+          }
+        return high;
       };
-      exponents();
-      bool grow = false;
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) grow |= y[n][i] > kHead + kLazy;
-      if (__any_sync(0xffffffffu, grow)) {
+      if (__any_sync(0xffffffffu, exponents() > kHead + kLazy)) {
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -463,8 +538,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
             // the scores themselves: y is too coarse beside m = kNone
             float top = m[n][e];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (y[n][2 * i + e] != -INFINITY) top = fmaxf(top, fmaf(sc[n][2 * i + e], f[n][e] * ks, lw));
+            for (int i = 0; i < kPages; ++i)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                if (y[i][n][2 * r + e] != -INFINITY) top = fmaxf(top, fmaf(sc[i][n][2 * r + e], f[n][e] * ks[i], lw[i]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const float alpha = exp2_fast(m[n][e] - top);
@@ -475,45 +552,60 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
           }
         exponents();
       }
-      uint32_t pb[kNT][2];
+      uint32_t pb[kPages][kNT][2];
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) {
+      for (int i = 0; i < kPages; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[n][i] = exp2_fast(y[n][i]);
-        l[n][0] = fmaf(y[n][0] + y[n][2], iw, l[n][0]);
-        l[n][1] = fmaf(y[n][1] + y[n][3], iw, l[n][1]);
-        pb[n][0] = movmatrix_trans(pack_half(y[n][0], y[n][1]));
-        pb[n][1] = movmatrix_trans(pack_half(y[n][2], y[n][3]));
-      }
-      if (kFp8 && masked) {
-        // Slots past the end may hold NaN patterns: 0 * NaN is not 0.
-        const int stop = bad ? 0 : seg.computed + seg.rows / a.group;
+        for (int n = 0; n < kNT; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (p * kPage + 2 * t + (i & 1) + (i >> 1) * 8 >= stop)
-#pragma unroll
-            for (int w = 0; w < kVWords; ++w) vreg[i][w] = 0;
-      }
+          for (int e = 0; e < 4; ++e) y[i][n][e] = exp2_fast(y[i][n][e]);
+          l[n][0] = fmaf(y[i][n][0] + y[i][n][2], iw[i], l[n][0]);
+          l[n][1] = fmaf(y[i][n][1] + y[i][n][3], iw[i], l[n][1]);
+          pb[i][n][0] = movmatrix_trans(pack_half(y[i][n][0], y[i][n][1]));
+          pb[i][n][1] = movmatrix_trans(pack_half(y[i][n][2], y[i][n][3]));
+        }
       // O: elements (D / 8) g + 2 j (rows g of the tile) and + 1 (rows g + 8).
+      cp_async_wait_group<1>();
 #pragma unroll
-      for (int w = 0; w < kVWords; ++w) {
+      for (int i = 0; i < kPages; ++i) {
+        const uint32_t src = ring + i * (2 * kSideBytes) + kSideBytes;
+        uint32_t vreg[4][kVWords];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // bytes (2 half, 2 half + 1) of value rows (0, 1) and (2, 3), interleaved
-          const uint32_t lo = P::bias(__byte_perm(vreg[0][w], vreg[1][w], half ? 0x7362 : 0x5140));
-          const uint32_t hi = P::bias(__byte_perm(vreg[2][w], vreg[3][w], half ? 0x7362 : 0x5140));
-          const uint32_t va[4] = {P::template get<false>(lo), P::template get<true>(lo), P::template get<false>(hi),
-                                  P::template get<true>(hi)};
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (D == 128)
+            lds_16(vreg[r], src + (r * 32 + lane) * 16);
+          else
+            lds_8(vreg[r], src + (r * 32 + lane) * 8);
+        }
+        if (kFp8 && masked) {
+          // Slots past the end may hold NaN patterns: 0 * NaN is not 0.
+          const int stop = now >> i & 1u ? seg.computed + seg.rows / a.group : 0;
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) mma_16816_nv<false>(o[n][2 * w + half], va, pb[n][0], pb[n][1]);
+          for (int r = 0; r < 4; ++r)
+            if ((p + i) * kPage + 2 * t + (r & 1) + (r >> 1) * 8 >= stop)
+#pragma unroll
+              for (int w = 0; w < kVWords; ++w) vreg[r][w] = 0;
+        }
+#pragma unroll
+        for (int w = 0; w < kVWords; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // bytes (2 half, 2 half + 1) of value rows (0, 1) and (2, 3), interleaved
+            const uint32_t lo = P::bias(__byte_perm(vreg[0][w], vreg[1][w], half ? 0x7362 : 0x5140));
+            const uint32_t hi = P::bias(__byte_perm(vreg[2][w], vreg[3][w], half ? 0x7362 : 0x5140));
+            const uint32_t va[4] = {P::template get<false>(lo), P::template get<true>(lo), P::template get<false>(hi),
+                                    P::template get<true>(hi)};
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) mma_16816_nv<false>(o[n][2 * w + half], va, pb[i][n][0], pb[i][n][1]);
+          }
         }
       }
-      // Everything of this slot is in registers and used: refill it.
-      if (slot == 0) fetch_next(0); else fetch_next(1);
-      slot ^= 1;
+      fetch_values();
     }
 
-    // The warps' sums.
+    // The warps' sums, kMeet warps at a time.
+    const bool whole = seg.first == 0 && seg.last == seg.pages;
+    const int piece = 2 * blockIdx.x + (seg.first == 0 ? 1 : 0);
 #pragma unroll
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -522,84 +614,108 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
         for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
         const int row = n * 8 + 2 * t + e;
         if (g == 0) m_sm[warp][row] = m[n][e], l_sm[warp][row] = l[n][e];
-        float *dst = o_sm + (warp * kRows + row) * Cfg::kPad + g * (D / 8);
-#pragma unroll
-        for (int j = 0; j < kDTiles; j += 2)
-          *reinterpret_cast<float4 *>(dst + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
       }
-    __syncthreads();
-    const bool whole = seg.first == 0 && seg.last == seg.pages;
-    const int piece = 2 * blockIdx.x + (seg.first == 0 ? 1 : 0);
-    auto store = [&](int row, int d, float4 v, float total_l) {
-      const float inv = total_l > 0.f ? 1.f / total_l : 0.f;
-      const int tok = row / a.group, head = row - tok * a.group;
-      uint16_t *dst = a.out + (seg.q0 + tok) * a.out_stride + (seg.kvh * a.group + head) * D + d;
-      if (a.out_vec) {
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<kBf16>(v.x * inv, v.y * inv), pack2<kBf16>(v.z * inv, v.w * inv));
-      } else {
-        dst[0] = from_float<kBf16>(v.x * inv), dst[1] = from_float<kBf16>(v.y * inv);
-        dst[2] = from_float<kBf16>(v.z * inv), dst[3] = from_float<kBf16>(v.w * inv);
+    auto put = [&]() {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float *dst = o_sm + ((warp % Cfg::kMeet) * kRows + n * 8 + 2 * t + e) * Cfg::kPad + g * (D / 8);
+#pragma unroll
+          for (int j = 0; j < kDTiles; j += 2)
+            *reinterpret_cast<float4 *>(dst + 2 * j) =
+                make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
+        }
+    };
+    // A warp adds up rows warp, warp + 8, ..: D / 4 lanes of 4 elements for each (two rows at once for D = 64).
+    constexpr int kLanes = D / 4, kSide = 32 / kLanes, kOwn = (kRows + kWarps * kSide - 1) / (kWarps * kSide);
+    const int d = lane % kLanes * 4;
+    float4 acc[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto take = [&](int from) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int row = (i * kWarps + warp) * kSide + lane / kLanes;
+        if (row >= rows) continue;
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_sm[w][row]);
+#pragma unroll
+        for (int w = 0; w < Cfg::kMeet; ++w) {
+          const float wt = exp2_fast(m_sm[from + w][row] - top);
+          const float4 v = *reinterpret_cast<const float4 *>(o_sm + (w * kRows + row) * Cfg::kPad + d);
+          acc[i].x = fmaf(wt, v.x, acc[i].x), acc[i].y = fmaf(wt, v.y, acc[i].y);
+          acc[i].z = fmaf(wt, v.z, acc[i].z), acc[i].w = fmaf(wt, v.w, acc[i].w);
+        }
       }
     };
-    for (int i = tid; i < seg.rows * (D / 4); i += kThreads) {
-      const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-      float top = kNone;
+    if (Cfg::kMeet == kWarps || warp < Cfg::kMeet) put();
+    __syncthreads();
+    take(0);
+    if constexpr (Cfg::kMeet < kWarps) {
+      __syncthreads();
+      if (warp >= Cfg::kMeet) put();
+      __syncthreads();
+      take(Cfg::kMeet);
+    }
+    auto store = [&](int row, float4 v, float total_l) {
+      const float inv = total_l == 0.f ? 0.f : 1.f / total_l;
+      const int tok = (row0 + row) / a.group, head = row0 + row - tok * a.group;
+      uint16_t *dst = a.out + (seg.q0 + tok) * a.out_stride + (seg.kvh * a.group + head) * D + d;
+      const uint32_t lo = pack2<kBf16>(v.x * inv, v.y * inv), hi = pack2<kBf16>(v.z * inv, v.w * inv);
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
+    };
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int row = (i * kWarps + warp) * kSide + lane / kLanes;
+      if (row >= rows) continue;
+      float top = kNone, sum_l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_sm[w][row]);
-      float sum_l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float wt = exp2_fast(m_sm[w][row] - top);
-        const float4 v = *reinterpret_cast<const float4 *>(o_sm + (w * kRows + row) * Cfg::kPad + d);
-        sum_l = fmaf(wt, l_sm[w][row], sum_l);
-        acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y);
-        acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
-      }
+      for (int w = 0; w < kWarps; ++w) sum_l = fmaf(exp2_fast(m_sm[w][row] - top), l_sm[w][row], sum_l);
       if (whole) {
-        store(row, d, acc, sum_l);
+        store(row, acc[i], sum_l);
       } else {
-        *reinterpret_cast<float4 *>(a.part_o + (static_cast<int64_t>(piece) * kMaxRows + row) * D + d) = acc;
-        if (d == 0) a.part_ml[piece * kMaxRows + row] = make_float2(top, sum_l);
+        const int64_t at = static_cast<int64_t>(piece) * kRows + row;
+        *reinterpret_cast<float4 *>(a.part_o + at * D + d) = acc[i];
+        if (d == 0) a.part_ml[at] = make_float2(top, sum_l);
       }
     }
     if (!whole) {
       // The CTAs that hold a piece of the item.
-      const long long item = end - left - seg.first;
-      const int c0 = static_cast<int>(item / run), c1 = static_cast<int>((item + seg.pages - 1) / run);
-      uint32_t *count = a.counts + c0;
+      const int c0 = static_cast<int>(seg.at / run), c1 = static_cast<int>((seg.at + seg.pages - 1) / run);
       __threadfence();
       __syncthreads();
-      if (tid == 0) last_sm = atomicAdd(count, 1u) == static_cast<uint32_t>(c1 - c0);
+      if (tid == 0) last_sm = atomicAdd(a.counts + c0, 1u) == static_cast<uint32_t>(c1 - c0);
       __syncthreads();
       if (last_sm) {
         __threadfence();
-        if (tid == 0) *count = 0;
-        for (int i = tid; i < seg.rows * (D / 4); i += kThreads) {
-          const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-          float top = kNone;
-          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(&a.part_ml[(2 * c + (c == c0)) * kMaxRows + row]).x);
-          float sum_l = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tid == 0) a.counts[c0] = 0;
+#pragma unroll 1
+        for (int row = warp * kSide + lane / kLanes; row < rows; row += kWarps * kSide) {
+          float top = kNone, sum_l = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          // Pieces in order, a few on their way; the sums move to a larger maximum as it comes.
 #pragma unroll 4
           for (int c = c0; c <= c1; ++c) {
-            const int at = (2 * c + (c == c0)) * kMaxRows + row;
-            const float2 ml = __ldcg(&a.part_ml[at]);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + static_cast<int64_t>(at) * D + d));
-            const float wt = exp2_fast(ml.x - top);
-            sum_l = fmaf(wt, ml.y, sum_l);
-            acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y);
-            acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
+            const int64_t at = static_cast<int64_t>(2 * c + (c == c0)) * kRows + row;
+            const float2 ml = __ldcg(a.part_ml + at);
+            const float4 u = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at * D + d));
+            const float grown = fmaxf(top, ml.x);
+            const float keep = exp2_fast(top - grown), wt = exp2_fast(ml.x - grown);
+            top = grown;
+            sum_l = fmaf(wt, ml.y, sum_l * keep);
+            v.x = fmaf(wt, u.x, v.x * keep), v.y = fmaf(wt, u.y, v.y * keep);
+            v.z = fmaf(wt, u.z, v.z * keep), v.w = fmaf(wt, u.w, v.w * keep);
           }
-          store(row, d, acc, sum_l);
+          store(row, v, sum_l);
         }
       }
     }
-    __syncthreads();  // o_sm is free again
-    Segment n;
-    more = next_segment(seg, n);
-    left -= seg.last - seg.first;
-    if (more) seg = n;
+    __syncthreads();  // the shared rows are free again
+    more = advance(walk_m);
   }
 }
 

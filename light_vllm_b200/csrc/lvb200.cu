@@ -2245,17 +2245,28 @@ struct Kv8Workspace {
 
 constexpr int kKv8DecodeCtasPerSm = 2;
 
-// Query rows of one KV head that the decode kernel takes: of every request if
-// the longest fits, else of single tokens beside prompt chunks.
-int kv8_few_rows(int64_t max_query_len, int64_t group) {
+// How the decode kernel takes a batch: tiles of 8 query rows of an item, and the
+// query rows of one KV head up to which a request is its: two row groups of every
+// request if the longest fits, else single tokens beside prompt chunks.  (Rows
+// above 64 read the cache a third time; from there the tile kernel is as fast.)
+struct Kv8Decode {
+  int tiles, few_rows;
+};
+
+Kv8Decode kv8_decode(int64_t max_query_len, int64_t group) {
+  constexpr int64_t kRows = lvb::kv8::kMaxRows;
   const int64_t rows = max_query_len * group;
-  const int64_t fit = rows <= lvb::kv8::kMaxRows ? rows : group;
-  return fit <= 8 ? 8 : fit <= lvb::kv8::kMaxRows ? lvb::kv8::kMaxRows : 0;
+  const int64_t fit = rows <= 2 * kRows ? rows : group;
+  if (fit > 2 * kRows) return {0, 0};
+  const int64_t groups = (fit + kRows - 1) / kRows, each = (fit + groups - 1) / groups;
+  const int tiles = static_cast<int>((each + 7) / 8);
+  return {tiles, static_cast<int>(groups) * tiles * 8};
 }
 
 Kv8Workspace kv8_workspace(int sms, bool tiles) {
   const size_t ctas = static_cast<size_t>(sms) * kKv8DecodeCtasPerSm;
-  const size_t rows = 2 * ctas * lvb::kv8::kMaxRows, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
+  // (two CTAs of 8 rows, or one of up to kMaxRows, for each SM)
+  const size_t rows = static_cast<size_t>(2) * sms * lvb::kv8::kMaxRows, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
   Kv8Workspace w{};
   w.tile_counts = round256(ctas * 4);
   w.o = w.tile_counts + round256(static_cast<size_t>(sms) * 4);
@@ -2300,7 +2311,7 @@ size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_hea
       current_device(&dev) != LVB_OK)
     return 0;
   const int64_t group = num_query_heads / num_kv_heads;
-  return kv8_workspace(sm_count(dev), max_query_len * group > kv8_few_rows(max_query_len, group)).total;
+  return kv8_workspace(sm_count(dev), max_query_len * group > kv8_decode(max_query_len, group).few_rows).total;
 }
 
 int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
@@ -2334,14 +2345,15 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
   a.value_scales = value_scales;
   a.hq = static_cast<int>(num_query_heads);
   a.group = static_cast<int>(num_query_heads / num_kv_heads);
-  a.query_vec = aligned16(query) && query_token_stride % 8 == 0;
-  a.out_vec = aligned16(out) && out_token_stride % 8 == 0;
+  if (!aligned16(query) || !aligned16(out) || query_token_stride % 8 || out_token_stride % 8)
+    return fail(LVB_ERR_INVALID, "kv8_attention: query and output rows must be 16-byte aligned");
   a.scale_log2 = scale * 1.4426950408889634f;
   if (max_query_len * a.group > INT_MAX) return fail(LVB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
   int dev = 0;
   rc = current_device(&dev);
   if (rc != LVB_OK) return rc;
-  a.few_rows = kv8_few_rows(max_query_len, a.group);
+  const Kv8Decode decode = kv8_decode(max_query_len, a.group);
+  a.few_rows = decode.few_rows;
   const bool tiles = max_query_len * a.group > a.few_rows;
   const Kv8Workspace w = kv8_workspace(sm_count(dev), tiles);
   if (workspace == nullptr || workspace_bytes < w.total || !aligned16(workspace))
@@ -2359,9 +2371,14 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
     constexpr int kD = decltype(d)::value;
     int status = LVB_OK;
     if (tiles) status = launch_kv8_tiles<kB16, kFp8, kD>(a, dev, st);
-    if (status == LVB_OK && a.few_rows == 8) status = launch_kv8_decode<kB16, kFp8, kD, 1>(a, dev, st);
-    if (status == LVB_OK && a.few_rows == 16) status = launch_kv8_decode<kB16, kFp8, kD, 2>(a, dev, st);
-    return status;
+    if (status != LVB_OK) return status;
+    switch (decode.tiles) {
+      case 1: return launch_kv8_decode<kB16, kFp8, kD, 1>(a, dev, st);
+      case 2: return launch_kv8_decode<kB16, kFp8, kD, 2>(a, dev, st);
+      case 3: return launch_kv8_decode<kB16, kFp8, kD, 3>(a, dev, st);
+      case 4: return launch_kv8_decode<kB16, kFp8, kD, 4>(a, dev, st);
+      default: return status;
+    }
   });
 }
 

@@ -134,6 +134,9 @@ at::Tensor fresh(at::IntArrayRef size, at::ScalarType type) {
                                               c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
 }
 
+// Whether rows may be read and written 16 bytes at a time.
+bool aligned(const at::Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % 8 == 0; }
+
 int act_of(const at::Tensor &t) {
   return t.scalar_type() == at::kHalf ? LVB_DTYPE_F16 : t.scalar_type() == at::kBFloat16 ? LVB_DTYPE_BF16 : -1;
 }
@@ -162,7 +165,8 @@ PyObject *attention(PyObject *const *args) {
   if (!q || q->dim() != 3 || !layer(args + 1, l) || !step(args + 5, l.device, s)) Py_RETURN_NONE;
   const int act = act_of(*q);
   const int64_t tokens = q->size(0), hq = q->size(1);
-  if (act < 0 || tokens == 0 || hq == 0 || l.hkv == 0 || hq % l.hkv || !rows(q, tokens, hq, l.d, q->scalar_type(), l.device))
+  if (act < 0 || tokens == 0 || hq == 0 || l.hkv == 0 || hq % l.hkv || !rows(q, tokens, hq, l.d, q->scalar_type(), l.device) ||
+      !aligned(*q))
     Py_RETURN_NONE;
   const double scale = PyFloat_AsDouble(args[10]);
   if (scale == -1.0 && PyErr_Occurred()) {
@@ -170,7 +174,7 @@ PyObject *attention(PyObject *const *args) {
     Py_RETURN_NONE;
   }
   const at::Tensor *given = args[11] == Py_None ? nullptr : tensor(args[11]);
-  if (args[11] != Py_None && !rows(given, tokens, hq, l.d, q->scalar_type(), l.device)) Py_RETURN_NONE;
+  if (args[11] != Py_None && (!rows(given, tokens, hq, l.d, q->scalar_type(), l.device) || !aligned(*given))) Py_RETURN_NONE;
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(l.device)).stream();
   Scratch ws;
   if (!scratch(kAttentionScratch, l.device, stream, g_attention_bytes(s.n, hq, l.hkv, l.d, s.max_query, s.max_seq), ws))

@@ -285,9 +285,11 @@ def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float
         out = torch.empty(query.shape, dtype=dtype, device=device)
     else:
         _check_rows("output", out, tokens, hq, d, dtype, index)
-        if _dense_heads(out) is not out:
-            raise KVCacheError("KV8 output rows must have dense heads")
+        if _dense_heads(out) is not out or out.data_ptr() % 16 or (tokens > 1 and out.stride(0) % 8):
+            raise KVCacheError("KV8 output rows must have dense heads and be 16-byte aligned")
     query = _dense_heads(query)
+    if query.data_ptr() % 16 or query.stride(0) % 8:
+        query = query.clone(memory_format=torch.contiguous_format)
     if tokens and n:
         with _on(index):
             lib = _native.library()
