@@ -39,6 +39,8 @@
 // counter for each item) sums them in order, so results do not depend on timing.
 #pragma once
 
+#include <type_traits>
+
 #include "kv8_cache.cuh"
 
 namespace lvb {
@@ -90,12 +92,36 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
+// Shared-memory loads and copies at constant offsets (in the instruction, not in
+// registers of their own).
+template <int kOff>
 __device__ __forceinline__ void lds_16(uint32_t (&v)[4], uint32_t src) {
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(src), "n"(kOff)
+               : "memory");
 }
 
+template <int kOff>
 __device__ __forceinline__ void lds_8(uint32_t (&v)[2], uint32_t src) {
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(src) : "memory");
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2 + %3];" : "=r"(v[0]), "=r"(v[1]) : "r"(src), "n"(kOff) : "memory");
+}
+
+template <int kBytes, int kDst, int kSrc>
+__device__ __forceinline__ void copy_at(uint32_t dst, const void *src) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(kDst), "n"(kSrc) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], 8;" ::"r"(dst), "l"(src), "n"(kDst), "n"(kSrc) : "memory");
+}
+
+// f(integral_constant 0), .., f(integral_constant N - 1)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F &&f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) { return pack2<false>(lo, hi); }
@@ -151,10 +177,6 @@ struct DecodeCfg {
   static constexpr int kScaleOff = kRingBytes + kOBytes + kQBytes;  // float [warp][page]{key, value}
   static constexpr int kSmemBytes = kScaleOff + kWarps * kPages * 8;
 };
-
-__device__ __forceinline__ void cp_async_8(uint32_t dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -323,7 +345,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
 
   // This lane's pieces of a page: 2 kKChunks of 16 bytes of K, four of 4 kVWords bytes of V.
   constexpr int kPages = Cfg::kPages, kSideBytes = Cfg::kSide;
-  const uint32_t ring = smem_u32(smem) + warp * (kPages * 2 * kSideBytes);  // [page][K, V]
+  const uint32_t ring = smem_u32(smem) + warp * (kPages * 2 * kSideBytes);  // [page][K, V][piece][lane]
+  const uint32_t ring16 = ring + lane * 16, ring_v = ring + kSideBytes + lane * (D / 8);
   const int ppb = s.bs / kPage;
   const uint32_t per_block = ppb > 1 ? 0xffffffffu / ppb + 1 : 0u;  // 2^32 / ppb, rounded up: exact for p * ppb < 2^32
   auto block_of = [&](int p) { return ppb == 1 ? p : static_cast<int>(__umulhi(p, per_block)); };
@@ -332,10 +355,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   // Scales come the same way: lane 2 i brings page i's key scale, 2 i + 1 its value scale.
   const uint32_t scale_ring = smem_u32(smem) + Cfg::kScaleOff + warp * (kPages * 8);
   const float *scale_lane = (lane & 1) == 0 ? a.key_scales : a.value_scales;
-  // The next step's pages (f_p .. of f_last, their KV head and table) and their
-  // blocks, read a step ahead so that no copy waits for them.
+  // The next step's pages (f_p .. of f_last, their KV head and table).  The blocks
+  // of the next 32 pages are in the lanes' f_ids, read in one go, so that no copy
+  // waits for its block.
   const int32_t *f_table = s.tables + walk_f.r * s.table_stride;
-  int f_p = walk_f.first + warp * kPages, f_last = walk_f.last, f_kvh = walk_f.kvh, f_phys[kPages];
+  int f_p = walk_f.first + warp * kPages, f_last = walk_f.last, f_kvh = walk_f.kvh, f_ids = 0, f_used = 32;
   asm volatile("" : "+l"(f_table), "+r"(f_last), "+r"(f_kvh));  // not to be read again from local memory
   bool f_more = true;
   uint32_t f_at[kPages];   // the pages' places, in pages of one head, for the values that follow the keys
@@ -348,11 +372,13 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       f_p = walk_f.first + warp * kPages;
       f_last = walk_f.last;
       f_kvh = walk_f.kvh;
+      f_used = 32;
       asm volatile("" : "+l"(f_table), "+r"(f_last), "+r"(f_kvh));
     }
-    if (f_more) {
-#pragma unroll
-      for (int i = 0; i < kPages; ++i) f_phys[i] = __ldg(f_table + block_of(min(f_p + i, f_last - 1)));
+    if (f_more && f_used == 32) {
+      const int p = f_p + lane / kPages * (kWarps * kPages) + lane % kPages;
+      f_ids = __ldg(f_table + block_of(min(p, f_last - 1)));
+      f_used = 0;
     }
   };
   auto fetch_keys = [&]() {
@@ -360,20 +386,20 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
     if (f_more) {
 #pragma unroll
       for (int i = 0; i < kPages; ++i) {
-        const bool bad = static_cast<uint32_t>(f_phys[i]) >= static_cast<uint32_t>(s.num_blocks);
-        const uint32_t h = bad ? 0u : static_cast<uint32_t>(f_phys[i]) * s.hkv + f_kvh;
+        const uint32_t phys = __shfl_sync(0xffffffffu, f_ids, f_used + i);
+        const bool bad = phys >= static_cast<uint32_t>(s.num_blocks);
+        const uint32_t h = bad ? 0u : phys * s.hkv + f_kvh;
         f_at[i] = (h - block_of(f_p + i)) * ppb + f_p + i;
         if (bad && f_p + i < f_last) record_device_error(LVB_DEVERR_INDEX);
         if (!bad && f_p + i < f_last) {
           f_there |= 1u << i;
           if (lane >> 1 == i) cp_async_4(scale_ring + lane * 4, scale_lane + h);
           const uint8_t *src = k_lane + static_cast<uint64_t>(f_at[i]) * kSideBytes;
-          const uint32_t dst = ring + i * (2 * kSideBytes);
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int c = 0; c < kKChunks; ++c)
-              cp_async_16(dst + ((r * kKChunks + c) * 32 + lane) * 16, src + r * 8 * D + c * 64, 16);
+          const uint32_t dst = ring16 + i * (2 * kSideBytes);
+          each<2 * kKChunks>([&](auto k) {
+            constexpr int kK = decltype(k)::value;
+            copy_at<16, kK * 512, kK / kKChunks * 8 * D + kK % kKChunks * 64>(dst, src);
+          });
         }
       }
     }
@@ -384,17 +410,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
     for (int i = 0; i < kPages; ++i)
       if (f_there >> i & 1u) {
         const uint8_t *src = v_lane + static_cast<uint64_t>(f_at[i]) * kSideBytes;
-        const uint32_t dst = ring + i * (2 * kSideBytes) + kSideBytes;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (D == 128)
-            cp_async_16(dst + (r * 32 + lane) * 16, src + ((r & 1) + (r >> 1) * 8) * D, 16);
-          else
-            cp_async_8(dst + (r * 32 + lane) * 8, src + ((r & 1) + (r >> 1) * 8) * D);
-        }
+        const uint32_t dst = ring_v + i * (2 * kSideBytes);
+        each<4>([&](auto r) {
+          constexpr int kR = decltype(r)::value;
+          copy_at<D / 8, kR * 32 * (D / 8), (kR % 2 + kR / 2 * 8) * D>(dst, src);
+        });
       }
     cp_async_commit();
     f_p += kWarps * kPages;
+    f_used += kPages;
     settle();
   };
   settle();
@@ -472,14 +496,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       float sc[kPages][kNT][4], ks[kPages], vs[kPages];
 #pragma unroll
       for (int i = 0; i < kPages; ++i) {
-        const uint32_t src = ring + i * (2 * kSideBytes);
+        const uint32_t src = ring16 + i * (2 * kSideBytes);
         uint32_t scales[2], kreg[2][kKChunks][4];
-        lds_8(scales, scale_ring + i * 8);
+        lds_8<0>(scales, scale_ring + i * 8);
         ks[i] = __uint_as_float(scales[0]), vs[i] = __uint_as_float(scales[1]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int c = 0; c < kKChunks; ++c) lds_16(kreg[r][c], src + ((r * kKChunks + c) * 32 + lane) * 16);
+        each<2 * kKChunks>([&](auto k) {
+          constexpr int kK = decltype(k)::value;
+          lds_16<kK * 512>(kreg[kK / kKChunks][kK % kKChunks], src);
+        });
 #pragma unroll
         for (int n = 0; n < kNT; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.f;
 #pragma unroll
@@ -568,15 +592,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       cp_async_wait_group<1>();
 #pragma unroll
       for (int i = 0; i < kPages; ++i) {
-        const uint32_t src = ring + i * (2 * kSideBytes) + kSideBytes;
+        const uint32_t src = ring_v + i * (2 * kSideBytes);
         uint32_t vreg[4][kVWords];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        each<4>([&](auto r) {
+          constexpr int kR = decltype(r)::value;
           if constexpr (D == 128)
-            lds_16(vreg[r], src + (r * 32 + lane) * 16);
+            lds_16<kR * 512>(vreg[kR], src);
           else
-            lds_8(vreg[r], src + (r * 32 + lane) * 8);
-        }
+            lds_8<kR * 256>(vreg[kR], src);
+        });
         if (kFp8 && masked) {
           // Slots past the end may hold NaN patterns: 0 * NaN is not 0.
           const int stop = now >> i & 1u ? seg.computed + seg.rows / a.group : 0;
