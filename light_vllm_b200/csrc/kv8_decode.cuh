@@ -162,16 +162,17 @@ struct Segment {
 // kNT: tiles of 8 query rows.
 template <int D, int kNT>
 struct DecodeCfg {
-  static constexpr int kWarps = 8;
+  // (Small CTAs, so that one's end of an item passes beside the others' pages.)
+  static constexpr int kWarps = kNT == 1 ? 4 : 8;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kCtasPerSm = kNT == 1 ? 2 : 1;
+  static constexpr int kCtasPerSm = kNT == 1 ? 4 : 1;
   static constexpr int kRows = 8 * kNT;
   static constexpr int kPad = D + 4;                // floats of a row of O in shared memory
   static constexpr int kPages = kNT <= 2 ? 2 : 1;   // pages of a step
   static constexpr int kSide = kPage * D;           // K (or V) of a page
   static constexpr int kRingBytes = kWarps * kPages * 2 * kSide;
-  // The warps' sums meet in shared memory kMeet warps at a time.
-  static constexpr int kMeet = kNT <= 1 ? 8 : 4;
+  // The warps' sums meet in shared memory in two halves.
+  static constexpr int kMeet = kWarps / 2;
   static constexpr int kOBytes = kMeet * kRows * kPad * 4;
   static constexpr int kQBytes = kNT == 1 ? 0 : kNT * (D / 16) * 32 * 8;  // query fragments
   static constexpr int kScaleOff = kRingBytes + kOBytes + kQBytes;  // float [warp][page]{key, value}
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   float *o_sm = reinterpret_cast<float *>(smem + Cfg::kRingBytes);                        // [kMeet][row][kPad]
   uint2 *q_sm = reinterpret_cast<uint2 *>(smem + Cfg::kRingBytes + Cfg::kOBytes);         // [kNT][kKSteps][32]
   __shared__ float m_sm[kWarps][kRows], l_sm[kWarps][kRows];
-  __shared__ long long scan[kWarps];
+  __shared__ longlong2 scan[kWarps];
   __shared__ Segment start_sm;
   __shared__ int last_sm;
   pdl_wait();
@@ -257,22 +258,22 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
     const int cost = (pages_of(q) + kItemCost + unit - 1) / unit * unit;
     return static_cast<long long>(cost) * ((q.n * a.group + kRows - 1) / kRows) * s.hkv;
   };
-  // Inclusive prefix over the CTA; `all` is the total.
-  auto block_scan = [&](long long v, long long &all) {
-    long long x = v;
+  // Inclusive prefix of two values over the CTA; `all` are the totals.
+  auto block_scan = [&](longlong2 v, longlong2 &all) {
+    longlong2 x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const long long y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
+      if (lane >= o) x.x += y, x.y += z;
     }
     __syncthreads();
     if (lane == 31) scan[warp] = x;
     __syncthreads();
-    all = 0;
+    all = make_longlong2(0, 0);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) x += scan[w];
-      all += scan[w];
+      if (w < warp) x.x += scan[w].x, x.y += scan[w].y;
+      all.x += scan[w].x, all.y += scan[w].y;
     }
     return x;
   };
@@ -281,29 +282,17 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   // Otherwise the flat order is cut into equal runs.
   constexpr int kSmallRun = kMinRun + kItemCost;
   Request mine{};
-  long long total = 0, padded = 0, sum, upto = 0;
+  longlong2 totals = make_longlong2(0, 0), sum, upto = totals;  // x: equal runs, y: pieces
 #pragma unroll 1
   for (int base = 0; base < s.num_seqs; base += kThreads) {
     mine.n = 0;
     if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
-    upto = block_scan(request_cost(mine, kSmallRun), sum);
-    padded += sum;
-    if (padded > static_cast<long long>(kSmallRun) * gridDim.x) break;
+    upto = block_scan(make_longlong2(request_cost(mine, 1), request_cost(mine, kSmallRun)), sum);
+    totals.x += sum.x;
+    totals.y += sum.y;
   }
-  const int unit = padded <= static_cast<long long>(kSmallRun) * gridDim.x ? kSmallRun : 1;
-  if (unit == 1) {
-#pragma unroll 1
-    for (int base = 0; base < s.num_seqs; base += kThreads) {
-      if (s.num_seqs > kThreads) {
-        mine.n = 0;
-        if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
-      }
-      upto = block_scan(request_cost(mine, 1), sum);
-      total += sum;
-    }
-  } else {
-    total = padded;
-  }
+  const int unit = totals.y <= static_cast<long long>(kSmallRun) * gridDim.x ? kSmallRun : 1;
+  const long long total = unit > 1 ? totals.y : totals.x;
   const long long run = unit > 1 ? unit : (total + gridDim.x - 1) / gridDim.x;
   const long long begin = run * blockIdx.x;
   if (begin >= total) return;
@@ -315,9 +304,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       if (s.num_seqs > kThreads) {
         mine.n = 0;
         if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
-        upto = block_scan(request_cost(mine, unit), sum);
+        upto = block_scan(make_longlong2(request_cost(mine, 1), request_cost(mine, kSmallRun)), sum);
       }
-      const long long hi = before + upto, lo = hi - request_cost(mine, unit);
+      const long long hi = before + (unit > 1 ? upto.y : upto.x), lo = hi - request_cost(mine, unit);
       if (lo <= begin && begin < hi) {
         // The run begins in one of this thread's request's items.
         const int pages = pages_of(mine), cost = (pages + kItemCost + unit - 1) / unit * unit, rows = mine.n * a.group;
@@ -335,7 +324,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
         seg.last = static_cast<int>(end - seg.at < pages ? (end > seg.at ? end - seg.at : 0) : pages);
         start_sm = seg;
       }
-      if (s.num_seqs > kThreads) before += sum;
+      if (s.num_seqs > kThreads) before += unit > 1 ? sum.y : sum.x;
     }
     __syncthreads();
   }
@@ -627,7 +616,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       fetch_values();
     }
 
-    // The warps' sums, kMeet warps at a time.
+    // The warps' sums, half of the warps at a time.
     const bool whole = seg.first == 0 && seg.last == seg.pages;
     const int piece = 2 * blockIdx.x + (seg.first == 0 ? 1 : 0);
 #pragma unroll
@@ -674,15 +663,13 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
         }
       }
     };
-    if (Cfg::kMeet == kWarps || warp < Cfg::kMeet) put();
+    if (warp < Cfg::kMeet) put();
     __syncthreads();
     take(0);
-    if constexpr (Cfg::kMeet < kWarps) {
-      __syncthreads();
-      if (warp >= Cfg::kMeet) put();
-      __syncthreads();
-      take(Cfg::kMeet);
-    }
+    __syncthreads();
+    if (warp >= Cfg::kMeet) put();
+    __syncthreads();
+    take(Cfg::kMeet);
     auto store = [&](int row, float4 v, float total_l) {
       const float inv = total_l == 0.f ? 0.f : 1.f / total_l;
       const int tok = (row0 + row) / a.group, head = row0 + row - tok * a.group;

@@ -2243,8 +2243,6 @@ struct Kv8Workspace {
   size_t counts, tile_counts, o, ml, tile_o, tile_ml, total;  // offsets
 };
 
-constexpr int kKv8DecodeCtasPerSm = 2;
-
 // How the decode kernel takes a batch: tiles of 8 query rows of an item, and the
 // query rows of one KV head up to which a request is its: two row groups of every
 // request if the longest fits, else single tokens beside prompt chunks.  (Rows
@@ -2263,12 +2261,12 @@ Kv8Decode kv8_decode(int64_t max_query_len, int64_t group) {
   return {tiles, static_cast<int>(groups) * tiles * 8};
 }
 
+constexpr int kKv8DecodeCtasPerSm = 4;  // at most, of 8 rows; one of up to kMaxRows
+
 Kv8Workspace kv8_workspace(int sms, bool tiles) {
-  const size_t ctas = static_cast<size_t>(sms) * kKv8DecodeCtasPerSm;
-  // (two CTAs of 8 rows, or one of up to kMaxRows, for each SM)
   const size_t rows = static_cast<size_t>(2) * sms * lvb::kv8::kMaxRows, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
   Kv8Workspace w{};
-  w.tile_counts = round256(ctas * 4);
+  w.tile_counts = round256(static_cast<size_t>(sms) * kKv8DecodeCtasPerSm * 4);
   w.o = w.tile_counts + round256(static_cast<size_t>(sms) * 4);
   w.ml = w.o + rows * 128 * sizeof(float);
   w.tile_o = round256(w.ml + rows * sizeof(float2));
@@ -2291,7 +2289,7 @@ int launch_kv8_tiles(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) 
 template <bool kBf16, bool kFp8, int D, int kNT>
 int launch_kv8_decode(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) {
   using Cfg = lvb::kv8::DecodeCfg<D, kNT>;
-  static_assert(Cfg::kCtasPerSm <= kKv8DecodeCtasPerSm, "workspace");
+  static_assert(Cfg::kCtasPerSm <= kKv8DecodeCtasPerSm && Cfg::kCtasPerSm * Cfg::kRows <= lvb::kv8::kMaxRows, "workspace");
   static bool smem_done[kMaxDevices] = {false};
   auto kernel = lvb::kv8::decode_kernel<kBf16, kFp8, D, kNT>;
   int rc = ensure_smem(kernel, Cfg::kSmemBytes, dev, smem_done);
