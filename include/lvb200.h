@@ -560,7 +560,7 @@ LVB_API int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, 
  * Query and output rows are 16-byte aligned (token strides multiples of 8).
  * Softmax statistics and sums in fp32.  max_query_len is the longest request
  * of the batch (LVB_DEVERR_INDEX and no output for a longer one); max_seq_len
- * guides how contexts are split and need not be exact.  workspace: the bytes
+ * (the longest context) bounds nothing and need not be exact.  workspace: the bytes
  * that lvb_kv8_attention_workspace_bytes gives for the same arguments (0:
  * none), 16-byte aligned, zero-filled once; every call leaves it as it needs
  * it.  Calls sharing a workspace must not overlap on the GPU. */

@@ -13,8 +13,12 @@ bytes of the 16-bit cache (runtime/execution/paged_cache.py:30-338, which has no
 * ``kv8_read_blocks`` -- values of whole blocks in the model's type
   (``lvb_kv8_read_blocks``);
 * ``KV8Cache`` and ``B200KV8AttentionBackend`` -- the same behind the contract
-  of ``B200PagedAttentionBackend``, so that ``Qwen2AWQRunner`` and light-vllm's
-  step handler run over the 8-bit cache unchanged.
+  of ``PagedAttentionBackend`` (runtime/execution/paged_attention.py:209-223):
+  a step's attention context for ``Qwen2AWQRunner`` or a ``ForwardBatch``.
+
+A block's scales only grow while the block is filled, drafted tokens that are
+refused later included: their slots are written over by the next step, but the
+step of the codes stays what the largest value needed.
 
 All of it runs on the current stream, allocates through torch and does not
 synchronise.  A call goes through ``_torch_ops`` (``csrc/torch_ops.cpp``), which
@@ -24,6 +28,8 @@ message and take whatever that hands back.
 
 from __future__ import annotations
 
+from collections.abc import Iterable
+from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
@@ -31,6 +37,8 @@ from torch import Tensor
 
 from light_vllm_b200 import _native
 from light_vllm_b200.kv_cache import KVCacheError
+from light_vllm_b200.paged_attention import StepMetadataPacker
+from light_vllm_b200.staging import SingleStepStaging
 
 _ACT_DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
 _CODE_DTYPES = {torch.int8: _native.KV8_INT8, torch.float8_e4m3fn: _native.KV8_E4M3}
@@ -49,8 +57,9 @@ class KV8Layer(NamedTuple):
 class KV8Step(NamedTuple):
     """A step's packed requests: int32 tensors on the device as
     ``lvb_pack_step_metadata`` lays them out, and two host numbers.
-    ``max_query_len`` is the longest request's query count; ``max_seq_len``
-    (computed and query tokens) guides how contexts are split."""
+    ``max_query_len`` is the longest request's query count, ``max_seq_len`` the
+    longest context (computed and query tokens); results do not depend on the
+    latter."""
 
     block_tables: Tensor  # [requests, blocks]
     num_computed: Tensor  # [requests], tokens cached by earlier steps
@@ -320,3 +329,160 @@ def _on(index: int):
     """The tensors' device made current (launches go to the current device)."""
 
     return _SAME if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+class KV8LayerSpec(NamedTuple):
+    """One attention layer's heads on this rank (``Qwen2AWQRunner.kv_layers()``)."""
+
+    layer_id: str
+    num_query_heads: int
+    num_kv_heads: int
+    head_size: int
+
+
+@dataclass(frozen=True, slots=True)
+class KV8CacheConfig:
+    """Geometry of a ``KV8Cache``; ``dtype`` is the type of its codes."""
+
+    num_blocks: int
+    block_size: int
+    dtype: torch.dtype = torch.int8
+    device: str | torch.device = "cuda"
+
+    def __post_init__(self) -> None:
+        if type(self.num_blocks) is not int or self.num_blocks <= 0:
+            raise ValueError("num_blocks must be a positive integer")
+        if type(self.block_size) is not int or self.block_size <= 0 or self.block_size % 16 or self.block_size > 1024:
+            raise ValueError("an 8-bit KV cache's block_size must be a multiple of 16 up to 1024")
+        if self.dtype not in _CODE_DTYPES:
+            raise ValueError("an 8-bit KV cache's dtype must be int8 or float8_e4m3fn")
+        object.__setattr__(self, "device", torch.device(self.device))
+
+
+class KV8Cache:
+    """The 8-bit counterpart of ``PagedKVCache``
+    (runtime/execution/paged_cache.py:328-338): zero-filled codes and scales of
+    every layer, reached through ``layer(layer_id)``.  Rows may be fp16 or bf16.
+
+    ``layers`` are (layer_id, query heads, KV heads, head size), as
+    ``Qwen2AWQRunner.kv_layers()`` gives them.  ``compact_kv`` does not take this
+    cache: accepted drafts of a linear layout need no move."""
+
+    def __init__(self, layers: Iterable[tuple[str, int, int, int]], config: KV8CacheConfig) -> None:
+        self.config = config
+        self._specs = {spec[0]: KV8LayerSpec(*spec) for spec in layers}
+        self._layers: dict[str, KV8Layer] = {}
+        for spec in self._specs.values():
+            if spec.head_size not in (64, 128):
+                raise ValueError("an 8-bit KV cache's head sizes are 64 and 128")
+            if spec.num_kv_heads <= 0 or spec.num_query_heads <= 0 or spec.num_query_heads % spec.num_kv_heads:
+                raise ValueError("num_query_heads must be a positive multiple of num_kv_heads")
+            codes = (config.num_blocks, spec.num_kv_heads, config.block_size, spec.head_size)
+            self._layers[spec.layer_id] = KV8Layer(
+                *(torch.zeros(codes, dtype=config.dtype, device=config.device) for _ in range(2)),
+                *(torch.zeros(codes[:2], dtype=torch.float32, device=config.device) for _ in range(2)))
+
+    @property
+    def layer_ids(self) -> tuple[str, ...]:
+        return tuple(self._specs)
+
+    def layer_spec(self, layer_id: str) -> KV8LayerSpec:
+        try:
+            return self._specs[layer_id]
+        except KeyError:
+            raise KVCacheError(f"unknown attention layer {layer_id!r}") from None
+
+    def layer(self, layer_id: str) -> KV8Layer:
+        self.layer_spec(layer_id)
+        return self._layers[layer_id]
+
+
+class B200KV8Attention:
+    """Per-step attention context over a ``KV8Cache``; one ``forward`` per layer.
+    ``step`` is the step's packed metadata."""
+
+    def __init__(self, cache: KV8Cache, step: KV8Step, num_tokens: int) -> None:
+        self.step = step
+        self._cache = cache
+        self._num_tokens = num_tokens
+        self._layer_ids: set[str] = set()
+
+    @property
+    def layer_ids(self) -> frozenset[str]:
+        return frozenset(self._layer_ids)
+
+    def forward(self, layer_id: str, query: Tensor, key: Tensor, value: Tensor, *, scale: float,
+                write_kv: bool = True) -> Tensor:
+        """Append this step's K/V to ``layer_id`` and return the attention output.
+
+        ``write_kv=False``: they are already in the cache (``rope_write_kv``)."""
+
+        if layer_id in self._layer_ids:
+            raise KVCacheError(f"paged attention layer {layer_id!r} ran more than once")
+        spec = self._cache.layer_spec(layer_id)
+        # The shape rules of the 16-bit backend (paged_attention.py:226-247).
+        if query.dim() != 3:
+            raise KVCacheError("paged attention query must have three dimensions")
+        if query.shape[0] != key.shape[0] or value.shape != key.shape:
+            raise KVCacheError("paged attention Q/K/V token dimensions must match")
+        if query.shape[0] != self._num_tokens:
+            raise KVCacheError("paged attention metadata token count does not match query")
+        if query.shape[1:] != (spec.num_query_heads, spec.head_size):
+            raise KVCacheError("paged attention query shape does not match the layer spec")
+        if key.shape[1:] != (spec.num_kv_heads, spec.head_size):
+            raise KVCacheError("paged attention K/V shape does not match the layer spec")
+        self._layer_ids.add(layer_id)
+        layer = self._cache.layer(layer_id)
+        if write_kv:
+            kv8_append(None, key, value, layer, self.step)
+        return kv8_attention(query, layer, self.step, scale=float(scale))
+
+    def rope_write_kv(self, layer_id: str, qkv: Tensor, q_heads: int, kv_heads: int, positions: Tensor,
+                      cos: Tensor, sin: Tensor) -> None:
+        """Rotate the query heads of merged QKV rows in place and append the
+        rotated keys and the values to ``layer_id``; follow with
+        ``forward(..., write_kv=False)``.  The key rows stay as they are."""
+
+        spec = self._cache.layer_spec(layer_id)
+        d = spec.head_size
+        if ((q_heads, kv_heads) != (spec.num_query_heads, spec.num_kv_heads) or qkv.dim() != 2
+                or qkv.shape != (self._num_tokens, (q_heads + 2 * kv_heads) * d)):
+            raise KVCacheError("QKV heads or tokens do not match the layer")
+        heads = qkv.unflatten(1, (-1, d))
+        query = heads[:, :q_heads]
+        kv8_append(query, heads[:, q_heads:q_heads + kv_heads], heads[:, q_heads + kv_heads:],
+                   self._cache.layer(layer_id), self.step, positions=positions, cos=cos, sin=sin, query_out=query)
+
+
+class B200KV8AttentionBackend:
+    """Creates one ``B200KV8Attention`` per model step, from light-vllm's own
+    ``PagedAttentionMetadata`` (linear layouts: a tree's rows see other positions
+    than their prefix).  The metadata is checked, packed and copied to the
+    device as ``B200PagedAttentionBackend`` does; the block-table rules and
+    their messages are the same."""
+
+    name = "b200-kv8"
+
+    def __init__(self) -> None:
+        _native.library()  # fail loudly at construction when the library is missing
+        self._packer = StepMetadataPacker()
+        self._staging: dict[torch.device, SingleStepStaging] = {}
+
+    def create(self, cache: KV8Cache, metadata) -> B200KV8Attention:
+        config = cache.config
+        device = config.device
+        if device.type != "cuda":
+            raise KVCacheError("B200 paged attention requires a CUDA KV cache")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        shape = self._packer.gather(metadata)
+        if not shape.linear:
+            raise KVCacheError("the 8-bit KV cache covers linear query layouts")
+        staging = self._staging.get(device)
+        if staging is None:
+            staging = self._staging[device] = SingleStepStaging(device)
+        packed = self._packer.stage(staging, config.num_blocks, config.block_size)
+        n, width = shape.num_seqs, shape.max_blocks
+        tables, computed, start = packed[:n * (width + 2) + 1].split((n * width, n, n + 1))
+        step = KV8Step(tables.view(n, width), computed, start, shape.max_query_len, shape.max_seq_len)
+        return B200KV8Attention(cache, step, shape.num_tokens)

@@ -287,7 +287,25 @@ class Qwen2AWQRunner:
         token of each row in ``logit_rows`` (every row when None).
 
         ``positions`` are int32 on the device; ``attention`` is an attention
-        context (``B200PagedAttention`` or ``StaticDecodeAttention``)."""
+        context (``B200PagedAttention``, ``B200KV8Attention`` or
+        ``StaticDecodeAttention``)."""
+
+        return self._greedy(self._hidden(input_ids, positions, attention, logit_rows))
+
+    def logits(self, input_ids: Tensor, positions: Tensor, attention, logit_rows: Tensor | None = None) -> Tensor:
+        """The step of ``forward``, returning the fp16 logits [rows, vocabulary]
+        (gathered over the vocabulary shards under tensor parallelism): what
+        sampling and the verification of drafts start from."""
+
+        local = torch.mm(self._hidden(input_ids, positions, attention, logit_rows), self.lm_head.t())
+        if self.world == 1:
+            return local
+        shards = torch.empty((self.world,) + tuple(local.shape), dtype=local.dtype, device=self.device)
+        dist.all_gather_into_tensor(shards, local, group=self.group)
+        return shards.transpose(0, 1).reshape(local.shape[0], -1)
+
+    def _hidden(self, input_ids: Tensor, positions: Tensor, attention, logit_rows: Tensor | None) -> Tensor:
+        """The decoder stack: final hidden rows of ``logit_rows`` (every row when None)."""
 
         s, lay = self.shape, self.layout
         t = input_ids.shape[0]
@@ -335,7 +353,7 @@ class Qwen2AWQRunner:
             x, residual = all_reduce_add_rms_norm(ws, down, residual, nxt, eps)
         if logit_rows is not None:
             x = x.index_select(0, logit_rows)
-        return self._greedy(x)
+        return x
 
     # ------------------------------------------------------------ CUDA graph
     def capture_decode(self, attention: "StaticDecodeAttention", ids: Tensor) -> "DecodeGraph":
