@@ -1,8 +1,8 @@
 // Attention of few query rows over the 8-bit paged cache: requests whose query
 // tokens times the query heads of one KV head are at most 64 (decode steps, and
-// the verification of a few drafts).  Up to 32 rows K and V are read once for all
-// of them, above by two row groups that follow each other (the second time from
-// L2).  Bound by those bytes.
+// the verification of a few drafts).  Up to 32 rows (40 for heads of 64) K and V
+// are read once for all of them, above by two row groups that follow each other
+// (the second time from L2).  Bound by those bytes.
 //
 // Mathematics.  With f_b = scale log2(e) key_scale_b and w_b = value_scale_b of
 // a position's block b, x_j = (q . key code_j) f_b + log2 w_b and a running
@@ -32,7 +32,7 @@
 // it lies in local memory.
 //
 // Split.  The pages of all (request, KV head, row group) items are laid end to
-// end, each item preceded by kItemCost pages' worth of what it costs besides, and
+// end, each item preceded by pages' worth of what it costs besides (kItemCost), and
 // cut into one equal run for each resident CTA, whatever the contexts' lengths;
 // the warps of a CTA take its pages in turn.  An item that ends in another CTA
 // leaves partial (O, m, L) in the workspace, and the last of its CTAs to finish (a
@@ -49,9 +49,11 @@ namespace kv8 {
 constexpr float kHead = 6.f;
 constexpr float kLazy = 8.f;
 constexpr int kPage = 16;     // positions a warp takes at a time
-constexpr int kMaxRows = 32;  // query rows of a decode item
-constexpr int kMinRun = 16;   // pages of a CTA, at least: more CTAs only merge more
-constexpr int kItemCost = 8;
+// Query rows of a decode item (their O in registers: 80 of them at 40 x 64).
+template <int D>
+constexpr int kMaxRows = D == 64 ? 40 : 32;
+constexpr int kMinRun = 16;    // pages of a CTA, at least: more CTAs only merge more
+constexpr int kSmallCost = 8;  // and pages' worth of an item's beginning there
 
 struct AttnArgs {
   Step step;
@@ -168,7 +170,10 @@ struct DecodeCfg {
   static constexpr int kCtasPerSm = kNT == 1 ? 4 : 1;
   static constexpr int kRows = 8 * kNT;
   static constexpr int kPad = D + 4;                // floats of a row of O in shared memory
-  static constexpr int kPages = kNT <= 2 ? 2 : 1;   // pages of a step
+  static constexpr int kPages = kNT <= (D == 64 ? 3 : 2) ? 2 : 1;  // pages of a step
+  // An item's queries, sums and joining in pages of the CTA's time.  (With 5 tiles
+  // of rows and heads of 64 they take 14K cycles and a page 280.)
+  static constexpr int kItemCost = kNT == 1 ? 8 : 40;
   static constexpr int kSide = kPage * D;           // K (or V) of a page
   static constexpr int kRingBytes = kWarps * kPages * 2 * kSide;
   // The warps' sums meet in shared memory in two halves.
@@ -197,11 +202,11 @@ __device__ __forceinline__ Request decode_request(const Step &s, int group, int 
 
 __device__ __forceinline__ int pages_of(const Request &q) { return (q.computed + q.n + kPage - 1) / kPage; }
 
-// To the run's next item with pages of the run; false at its end.  `left` rows of
-// the flat order are walked in steps of an item's cost, rounded up to `unit`.
-__device__ __noinline__ bool next_item(const Step &s, int group_heads, int few_rows, int rows_each, int unit, long long end,
-                                       Segment &seg) {
-  const int cost = (seg.pages + kItemCost + unit - 1) / unit * unit;
+// To the run's next item with pages of the run; false at its end.  The flat order
+// is walked in steps of an item's cost, its pages and `more`, rounded up to `unit`.
+__device__ __noinline__ bool next_item(const Step &s, int group_heads, int few_rows, int rows_each, int unit, int more,
+                                       long long end, Segment &seg) {
+  const int cost = (seg.pages + more + unit - 1) / unit * unit;
   const long long at = seg.at + cost;
   if (at >= end) return false;
   int r = seg.r, kvh = seg.kvh, group = seg.group + 1;
@@ -253,9 +258,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   const int g = lane >> 2, t = lane & 3;
 
   // What the items of a request come to (rounded up to `unit` each).
-  auto request_cost = [&](const Request &q, int unit) {
+  auto request_cost = [&](const Request &q, int unit, int more) {
     if (q.n == 0) return 0ll;
-    const int cost = (pages_of(q) + kItemCost + unit - 1) / unit * unit;
+    const int cost = (pages_of(q) + more + unit - 1) / unit * unit;
     return static_cast<long long>(cost) * ((q.n * a.group + kRows - 1) / kRows) * s.hkv;
   };
   // Inclusive prefix of two values over the CTA; `all` are the totals.
@@ -280,18 +285,19 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   // A batch that gives every CTA at most kSmallRun pages is cut at the items'
   // starts: a piece each for the CTAs, and short items are not cut at all.
   // Otherwise the flat order is cut into equal runs.
-  constexpr int kSmallRun = kMinRun + kItemCost;
+  constexpr int kItemCost = Cfg::kItemCost, kSmallRun = kMinRun + kSmallCost;
   Request mine{};
   longlong2 totals = make_longlong2(0, 0), sum, upto = totals;  // x: equal runs, y: pieces
 #pragma unroll 1
   for (int base = 0; base < s.num_seqs; base += kThreads) {
     mine.n = 0;
     if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
-    upto = block_scan(make_longlong2(request_cost(mine, 1), request_cost(mine, kSmallRun)), sum);
+    upto = block_scan(make_longlong2(request_cost(mine, 1, kItemCost), request_cost(mine, kSmallRun, kSmallCost)), sum);
     totals.x += sum.x;
     totals.y += sum.y;
   }
   const int unit = totals.y <= static_cast<long long>(kSmallRun) * gridDim.x ? kSmallRun : 1;
+  const int item_cost = unit > 1 ? kSmallCost : kItemCost;
   const long long total = unit > 1 ? totals.y : totals.x;
   const long long run = unit > 1 ? unit : (total + gridDim.x - 1) / gridDim.x;
   const long long begin = run * blockIdx.x;
@@ -304,18 +310,18 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       if (s.num_seqs > kThreads) {
         mine.n = 0;
         if (base + tid < s.num_seqs) mine = decode_request(s, a.group, a.few_rows, base + tid);
-        upto = block_scan(make_longlong2(request_cost(mine, 1), request_cost(mine, kSmallRun)), sum);
+        upto = block_scan(make_longlong2(request_cost(mine, 1, kItemCost), request_cost(mine, kSmallRun, kSmallCost)), sum);
       }
-      const long long hi = before + (unit > 1 ? upto.y : upto.x), lo = hi - request_cost(mine, unit);
+      const long long hi = before + (unit > 1 ? upto.y : upto.x), lo = hi - request_cost(mine, unit, item_cost);
       if (lo <= begin && begin < hi) {
         // The run begins in one of this thread's request's items.
-        const int pages = pages_of(mine), cost = (pages + kItemCost + unit - 1) / unit * unit, rows = mine.n * a.group;
+        const int pages = pages_of(mine), cost = (pages + item_cost + unit - 1) / unit * unit, rows = mine.n * a.group;
         const int item = static_cast<int>((begin - lo) / cost), groups = (rows + kRows - 1) / kRows;
         Segment seg;
         seg.r = base + tid;
         seg.kvh = item / groups;
         seg.group = item % groups;
-        seg.at = lo + static_cast<long long>(item) * cost + kItemCost;
+        seg.at = lo + static_cast<long long>(item) * cost + item_cost;
         seg.q0 = mine.q0;
         seg.rows = rows;
         seg.computed = mine.computed;
@@ -330,7 +336,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
   }
   // Walked twice, by the page loop and, ahead of it, by the copies.
   Segment walk_m = start_sm, walk_f = walk_m;
-  auto advance = [&](Segment &walk) { return next_item(s, a.group, a.few_rows, kRows, unit, end, walk); };
+  auto advance = [&](Segment &walk) { return next_item(s, a.group, a.few_rows, kRows, unit, item_cost, end, walk); };
 
   // This lane's pieces of a page: 2 kKChunks of 16 bytes of K, four of 4 kVWords bytes of V.
   constexpr int kPages = Cfg::kPages, kSideBytes = Cfg::kSide;

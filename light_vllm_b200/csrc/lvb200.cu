@@ -2251,11 +2251,12 @@ struct Kv8Decode {
   int tiles, few_rows;
 };
 
-Kv8Decode kv8_decode(int64_t max_query_len, int64_t group) {
-  constexpr int64_t kRows = lvb::kv8::kMaxRows;
+Kv8Decode kv8_decode(int64_t max_query_len, int64_t group, int64_t d) {
+  constexpr int64_t kFew = 64;
+  const int64_t kRows = d == 64 ? lvb::kv8::kMaxRows<64> : lvb::kv8::kMaxRows<128>;
   const int64_t rows = max_query_len * group;
-  const int64_t fit = rows <= 2 * kRows ? rows : group;
-  if (fit > 2 * kRows) return {0, 0};
+  const int64_t fit = rows <= kFew ? rows : group;
+  if (fit > kFew) return {0, 0};
   const int64_t groups = (fit + kRows - 1) / kRows, each = (fit + groups - 1) / groups;
   const int tiles = static_cast<int>((each + 7) / 8);
   return {tiles, static_cast<int>(groups) * tiles * 8};
@@ -2264,7 +2265,7 @@ Kv8Decode kv8_decode(int64_t max_query_len, int64_t group) {
 constexpr int kKv8DecodeCtasPerSm = 4;  // at most, of 8 rows; one of up to kMaxRows
 
 Kv8Workspace kv8_workspace(int sms, bool tiles) {
-  const size_t rows = static_cast<size_t>(2) * sms * lvb::kv8::kMaxRows, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
+  const size_t rows = static_cast<size_t>(2) * sms * lvb::kv8::kMaxRows<64>, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
   Kv8Workspace w{};
   w.tile_counts = round256(static_cast<size_t>(sms) * kKv8DecodeCtasPerSm * 4);
   w.o = w.tile_counts + round256(static_cast<size_t>(sms) * 4);
@@ -2289,7 +2290,7 @@ int launch_kv8_tiles(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) 
 template <bool kBf16, bool kFp8, int D, int kNT>
 int launch_kv8_decode(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream) {
   using Cfg = lvb::kv8::DecodeCfg<D, kNT>;
-  static_assert(Cfg::kCtasPerSm <= kKv8DecodeCtasPerSm && Cfg::kCtasPerSm * Cfg::kRows <= lvb::kv8::kMaxRows, "workspace");
+  static_assert(Cfg::kCtasPerSm <= kKv8DecodeCtasPerSm && Cfg::kCtasPerSm * Cfg::kRows <= lvb::kv8::kMaxRows<64>, "workspace");
   static bool smem_done[kMaxDevices] = {false};
   auto kernel = lvb::kv8::decode_kernel<kBf16, kFp8, D, kNT>;
   int rc = ensure_smem(kernel, Cfg::kSmemBytes, dev, smem_done);
@@ -2303,13 +2304,13 @@ int launch_kv8_decode(const lvb::kv8::AttnArgs &a, int dev, cudaStream_t stream)
 
 size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
                                          int64_t head_size, int64_t max_query_len, int64_t max_seq_len) {
-  (void)head_size, (void)max_seq_len;
+  (void)max_seq_len;
   int dev = 0;
   if (num_seqs <= 0 || num_kv_heads <= 0 || num_query_heads <= 0 || max_query_len <= 0 || max_query_len > INT_MAX ||
       current_device(&dev) != LVB_OK)
     return 0;
   const int64_t group = num_query_heads / num_kv_heads;
-  return kv8_workspace(sm_count(dev), max_query_len * group > kv8_decode(max_query_len, group).few_rows).total;
+  return kv8_workspace(sm_count(dev), max_query_len * group > kv8_decode(max_query_len, group, head_size).few_rows).total;
 }
 
 int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
@@ -2350,7 +2351,7 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
   int dev = 0;
   rc = current_device(&dev);
   if (rc != LVB_OK) return rc;
-  const Kv8Decode decode = kv8_decode(max_query_len, a.group);
+  const Kv8Decode decode = kv8_decode(max_query_len, a.group, head_size);
   a.few_rows = decode.few_rows;
   const bool tiles = max_query_len * a.group > a.few_rows;
   const Kv8Workspace w = kv8_workspace(sm_count(dev), tiles);
@@ -2375,6 +2376,9 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
       case 2: return launch_kv8_decode<kB16, kFp8, kD, 2>(a, dev, st);
       case 3: return launch_kv8_decode<kB16, kFp8, kD, 3>(a, dev, st);
       case 4: return launch_kv8_decode<kB16, kFp8, kD, 4>(a, dev, st);
+      case 5:
+        if constexpr (kD == 64) return launch_kv8_decode<kB16, kFp8, kD, 5>(a, dev, st);
+        return status;
       default: return status;
     }
   });
