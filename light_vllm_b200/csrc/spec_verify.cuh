@@ -56,7 +56,9 @@ constexpr int kScratchWords = kMaxChunks * kWarps + 2;  // of 8 bytes
 // its segments' weights, and the last one to finish finds the segment and then
 // the token at which the prefix sum passes the bar.  Bound by reading one row (two
 // after a refusal) of the vocabulary once; a call of one request by the latency
-// of its dependent loads.
+// of its dependent loads.  64 requests of 4 drafts over 152064 words: 21 us, 45 %
+// of the measured copy rate's (27 us with a block scan for every chunk, 110 us with
+// one CTA a request); one request: 6 us.
 __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_wait();
   __shared__ int stop_sm, last_sm, found_sm, segment_sm;
