@@ -593,7 +593,8 @@ LVB_API int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride,
  * num_accepted: drafts accepted.  A request without rows, with rows outside
  * the batch or with more than max_query_len sets LVB_DEVERR_INDEX and gets -1
  * throughout and 0 accepted.  A drafted token outside the vocabulary is refused and sets
- * LVB_DEVERR_INDEX.  Weights that are NaN or negative count as 0.
+ * LVB_DEVERR_INDEX.  Weights that are NaN or negative count as 0.  Up to 2^22
+ * words (LVB_ERR_UNSUPPORTED above).
  * workspace: lvb_verify_drafts_workspace_bytes() bytes (0: none), 16-byte
  * aligned, zero-filled once; calls sharing one must not overlap on the GPU.
  * The reference accepts drafts by greedy comparison only

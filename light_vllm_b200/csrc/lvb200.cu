@@ -2397,6 +2397,9 @@ int lvb_verify_drafts(const float *target_probs, int64_t target_stride, const fl
   if (num_seqs < 0 || num_seqs > 65535 || num_rows < 0 || num_rows > INT_MAX || max_query_len < 0 ||
       max_query_len > INT_MAX || vocab_size <= 0 || vocab_size > INT_MAX)
     return fail(LVB_ERR_INVALID, "verify_drafts: invalid batch or vocabulary size");
+  // (the weights' sum, in whole numbers of 2^-40, has 63 bits)
+  if (vocab_size > (int64_t{1} << 22))
+    return fail(LVB_ERR_UNSUPPORTED, "verify_drafts: %lld words (up to 2^22 are covered)", (long long)vocab_size);
   if (num_seqs == 0) return LVB_OK;
   if (num_rows < num_seqs) return fail(LVB_ERR_INVALID, "verify_drafts: every request needs a row");
   if (target_stride < vocab_size || (draft_probs && draft_stride < vocab_size))

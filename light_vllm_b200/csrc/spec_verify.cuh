@@ -9,7 +9,8 @@
 // exactly.
 //
 // The draw inverts the distribution function at a given uniform number in
-// whole numbers: W_v = round(2^40 min(w_v, 1)) (0 for w_v <= 0 and NaN), bar =
+// whole numbers: W_v = round(2^40 min(w_v, 1)) (0 for w_v <= 0 and NaN; the sum
+// of 2^22 words at most fits 63 bits), bar =
 // floor(u sum W), token = the lowest v whose prefix sum exceeds bar.  Sums of
 // whole numbers are the same in every order, so the token does not depend on
 // how the vocabulary is split.  A weight below 2^-41 is never drawn.  If every
@@ -36,9 +37,31 @@ struct VerifyArgs {
   unsigned long long *scratch;
 };
 
+// W of a weight w in [0, 1] as hi 2^20 + lo, by four additions (a conversion to 64
+// bits takes some twenty instructions): w 2^40 + 1.5 2^43 is rounded to a multiple
+// of 2^20, which its low bits then hold; what is left is below 2^20 and rounds to
+// a whole number in the same way (ties to even: hi 2^20 is even).  Both parts are
+// held with their constants' bits on top, and sums of them are taken modulo 2^32.
+struct Fixed {
+  static constexpr float kHi = 1.5f * 0x1p43f, kLo = 1.5f * 0x1p23f;
+  static constexpr uint32_t kHiBits = 0x55400000u, kLoBits = 0x4b400000u;
+  uint32_t hi = 0, lo = 0;
+  __device__ __forceinline__ void add(float w) {
+    const float h = __fmaf_rn(w, 0x1p40f, kHi);
+    hi += __float_as_uint(h);
+    lo += __float_as_uint(__fadd_rn(__fmaf_rn(w, 0x1p40f, -__fadd_rn(h, -kHi)), kLo));
+  }
+  // The sum of `count` weights, up to 2^10 of them.
+  __device__ __forceinline__ long long value(uint32_t count) const {
+    return (static_cast<long long>(static_cast<int32_t>(hi - count * kHiBits)) << 20) +
+           static_cast<int32_t>(lo - count * kLoBits);
+  }
+};
+
 __device__ __forceinline__ long long fixed_weight(float w) {
-  w = w > 0.f ? fminf(w, 1.f) : 0.f;
-  return __float2ll_rn(w * 0x1p40f);
+  Fixed f;
+  f.add(w);
+  return f.value(1);
 }
 
 // The vocabulary is cut into segments, one for each warp; a CTA of kWarps warps
@@ -56,9 +79,10 @@ constexpr int kScratchWords = kMaxChunks * kWarps + 2;  // of 8 bytes
 // its segments' weights, and the last one to finish finds the segment and then
 // the token at which the prefix sum passes the bar.  Bound by reading one row (two
 // after a refusal) of the vocabulary once; a call of one request by the latency
-// of its dependent loads.  64 requests of 4 drafts over 152064 words: 21 us, 45 %
-// of the measured copy rate's (27 us with a block scan for every chunk, 110 us with
-// one CTA a request); one request: 6 us.
+// of its dependent loads.  64 requests of 4 drafts over 152064 words: 19.5 us, 49 %
+// of the measured copy rate's (21.0 us with conversions to 64 bits, 27 us with a
+// block scan for every chunk as well, 110 us with one CTA a request); one request:
+// 6 us.
 __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(const __grid_constant__ VerifyArgs a) {
   pdl_wait();
   __shared__ int stop_sm, last_sm, found_sm, segment_sm;
@@ -113,8 +137,9 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
   // where it lies the same way.
   const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 2 & 3);
   const bool alike = q == nullptr || static_cast<int>(reinterpret_cast<uintptr_t>(q) >> 2 & 3) == shift;
-  auto weights = [&](int v, int lo, int hi, bool residual, long long (&w)[4]) {
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+  auto weights = [&](int v, int lo, int hi, bool residual, float (&x)[4]) {
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    x[0] = x[1] = x[2] = x[3] = 0.f;
     const bool less = residual && q != nullptr;
     if (v >= lo && v + 4 <= hi) {
       const float4 t = __ldg(reinterpret_cast<const float4 *>(p + v));
@@ -135,18 +160,30 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = residual && v + i == gone ? 0ll : fixed_weight(less ? __fsub_rn(x[i], y[i]) : x[i]);
+    for (int i = 0; i < 4; ++i) x[i] = __saturatef(__fsub_rn(x[i], y[i]));  // (NaN: 0)
   };
   auto group_start = [&](int v) { return (v + shift) / 4 * 4 - shift; };
   // Sum over [v0, v1) by one warp (every lane's result).
   auto warp_sum_of = [&](int v0, int v1, bool residual) {
     long long own = 0;
-#pragma unroll 4
-    for (int v = group_start(v0) + lane * 4; v < v1; v += 128) {
-      long long w[4];
-      weights(v, v0, v1, residual, w);
-      own += (w[0] + w[1]) + (w[2] + w[3]);
+    constexpr int kTogether = 4;
+    int v = group_start(v0) + lane * 4;
+#pragma unroll 1
+    for (; v < v1; v += kTogether * 128) {
+      float x[kTogether][4];
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+        if (v + i * 128 < v1) weights(v + i * 128, v0, v1, residual, x[i]);
+      }
+      Fixed f;
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.add(x[i][k]);
+      own += f.value(4 * kTogether);
     }
+    if (residual && lane == 0 && gone >= v0 && gone < v1) own -= fixed_weight(__saturatef(__ldg(p + gone)));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
     return own;
@@ -228,8 +265,11 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
     const int lo = segment_sm * a.segment, hi = min(a.vocab, lo + a.segment);
     for (int v = group_start(lo); v < hi; v += kVerifyThreads * 4) {
       const int own_v = v + tid * 4;
-      long long w[4] = {0, 0, 0, 0}, all;
-      if (own_v < hi) weights(own_v, lo, hi, residual, w);
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      long long w[4], all;
+      if (own_v < hi) weights(own_v, lo, hi, residual, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = residual && own_v + i == gone ? 0ll : fixed_weight(x[i]);
       own = (w[0] + w[1]) + (w[2] + w[3]);
       const long long mine_upto = block_prefix(own, all);
       if (before + all > bar) {  // the token is here

@@ -124,3 +124,10 @@ def test_read_and_verify_entries():
         assert verify(**change) == _native.LVB_ERR_INVALID
         assert message in lib.lvb_last_error()
     assert verify(n=0) == _native.LVB_OK
+
+
+def test_verification_of_more_words_than_its_sums_hold():
+    lib = _native.library()
+    words = (1 << 22) + 1
+    assert lib.lvb_verify_drafts(16, words, None, 0, None, None, 16, 16, 16, 16, 1, 1, 2, words, None, 0, None) == _native.LVB_ERR_UNSUPPORTED
+    assert b"2^22" in lib.lvb_last_error()
