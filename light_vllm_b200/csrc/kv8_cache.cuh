@@ -188,13 +188,35 @@ __device__ __forceinline__ void rotate(float (&x)[16], const Turn &t) {
   }
 }
 
+// Code<kFp8>::encode of four values, in fewer instructions: NaN passes the lower
+// bound and becomes 0 in the conversion to int32, packing saturates to 127; the
+// conversion to e4m3 saturates by itself.
+template <bool kFp8>
+__device__ __forceinline__ uint32_t encode_four(float x0, float x1, float x2, float x3) {
+  if constexpr (kFp8) {
+    auto known = [](float x) { return x == x ? x : 0.f; };
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(known(x0), known(x1)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(known(x2), known(x3)), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  } else {
+    auto whole = [](float x) {
+      float y;
+      asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(y) : "f"(x));  // -127
+      return __float2int_rn(y);
+    };
+    uint32_t hi, all;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(hi) : "r"(whole(x3)), "r"(whole(x2)), "r"(0));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(whole(x1)), "r"(whole(x0)), "r"(hi));
+    return all;
+  }
+}
+
 template <bool kFp8>
 __device__ __forceinline__ uint2 encode_piece(const float *x, float inv) {
-  uint32_t w[2] = {0, 0};
+  float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    w[i >> 2] |= static_cast<uint32_t>(Code<kFp8>::encode(__fmul_rn(x[i], inv))) << (8 * (i & 3));
-  return make_uint2(w[0], w[1]);
+  for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[i], inv);
+  return make_uint2(encode_four<kFp8>(y[0], y[1], y[2], y[3]), encode_four<kFp8>(y[4], y[5], y[6], y[7]));
 }
 
 constexpr int kAppendThreads = 128;
