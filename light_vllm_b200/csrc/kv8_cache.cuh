@@ -229,8 +229,9 @@ constexpr int kAppendThreads = 128;
 // its rotation is read once.  Bound by the bytes of the rows: every access is 16
 // (codes: 8) bytes a lane, and rows are asked for before anything that they do
 // not depend on.  Four prompts of 2048 tokens (40/8 heads of 128, bf16 to int8) with
-// the reading back of their blocks: 67 us, 4.1 TB/s (92 us with the block's rows
-// rotated before they are held, 122 us with 2-byte accesses).
+// the reading back of their blocks: 66 us, 4.2 TB/s (92 us with the block's rows
+// rotated before they are held, 122 us with 2-byte accesses; 78 us with these CTAs
+// spread among the queries').
 template <bool kBf16, bool kFp8, int D>
 __global__ void __launch_bounds__(kAppendThreads, 6) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
