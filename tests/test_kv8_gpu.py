@@ -415,3 +415,20 @@ def test_out_of_range_metadata_is_reported_and_left_out():
         assert torch.equal(x, y)
     got = kv8_read_blocks(layer, torch.tensor([9, 1], dtype=torch.int32, device=DEV), dtype=torch.float16)
     assert _native.device_error() == 2 and not got[0][0].any() and got[0][1].any()
+
+
+@pytest.mark.parametrize("heads,query", [((14, 2, 64), 8), ((14, 2, 64), 9), ((16, 1, 64), 3), ((64, 1, 64), 1), ((16, 1, 128), 4),
+                                         ((28, 4, 128), 6), ((64, 1, 128), 1), ((24, 8, 64), 13), ((33, 1, 64), 1)], ids=str)
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attention_of_rows_in_two_groups(heads, query, code):
+    """33 to 64 query rows of a KV head: one or two groups of the decode kernel's."""
+
+    requests = [(700, query), (0, query), (15, 1), (2040, max(1, query - 1)), (64, 0), (333, query)]
+    hq, hkv, d = heads
+    tables, blocks = _tables(requests, 16, seed=3)
+    layer = _layer(blocks, hkv, 16, d, code, seed=4)
+    step = _step(tables, requests)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    query_rows = torch.randn((sum(n for _, n in requests), hq, d), device=DEV, generator=gen).to(torch.bfloat16)
+    out = kv8_attention(query_rows, layer, step, scale=d ** -0.5)
+    _check_attention(query_rows, layer, step, tables, requests, code, d ** -0.5, out)
