@@ -161,3 +161,26 @@ def test_emitted_tokens_follow_the_target(probs):
     assert (second[~taken] == -1).all()
     count, m = np.bincount(second[taken], minlength=vocab), taken.sum()
     assert (np.abs(count - m * p) <= 5 * np.sqrt(m * p * (1 - p)) + 1e-6).all()
+
+
+@pytest.mark.parametrize("kind", ["halves", "small", "steps", "wide", "ones"])
+def test_weights_become_whole_numbers_by_the_rule(kind):
+    """Draws from weights whose whole numbers show how they were rounded."""
+
+    rng = np.random.default_rng(7)
+    rows, vocab = 96, 5000
+    if kind == "halves":  # ties: to the even neighbour
+        target = (rng.integers(0, 64, (rows, vocab)) + 0.5) * 2.0 ** -40
+    elif kind == "small":  # around half of the least weight, and far below
+        target = np.exp2(rng.uniform(-60, -38, (rows, vocab)))
+    elif kind == "steps":  # at the multiples of 2^-20 where the parts of a weight meet
+        target = (rng.integers(0, 9, (rows, vocab)) + rng.choice([-0.5, 0.0, 0.5], (rows, vocab))) * 2.0 ** -20
+        target = np.abs(target + rng.integers(-3, 4, (rows, vocab)) * 2.0 ** -40)
+    elif kind == "wide":
+        target = np.exp2(rng.uniform(-45, 0, (rows, vocab)))
+    else:
+        target = np.ones((rows, vocab))
+    target = target.astype(np.float32)
+    none = np.zeros(0, np.float32)
+    start = np.arange(rows + 1, dtype=np.int32)
+    _check((target, np.zeros(0, np.int64), none, rng.random(rows, dtype=np.float32), start, None))
