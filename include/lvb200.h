@@ -533,7 +533,9 @@ enum lvb_kv8_code { LVB_KV8_INT8 = 0, LVB_KV8_E4M3 = 1 };
  * for e4m3), earlier tokens' codes are rounded anew if the scale grew, and
  * the new tokens' codes are round(x / scale).  Slots past the request's end
  * are left as they are.  A block must not be shared by requests that write
- * to it (the rule of lvb_pack_step_metadata). */
+ * to it (the rule of lvb_pack_step_metadata).  The table has table_stride
+ * columns; lvb_kv8_append_strided takes the columns and the row stride apart
+ * (columns of a wider buffer; stride 0: one row for every request). */
 LVB_API int lvb_kv8_append(const uint16_t *query, int64_t query_token_stride, uint16_t *query_out,
                            int64_t query_out_stride, const uint16_t *key, int64_t key_token_stride,
                            const uint16_t *value, int64_t value_token_stride, const int32_t *positions,
@@ -543,6 +545,16 @@ LVB_API int lvb_kv8_append(const uint16_t *query, int64_t query_token_stride, ui
                            int64_t num_seqs, int64_t num_tokens, int64_t max_query_len, int64_t num_query_heads,
                            int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks, int dtype,
                            int code_type, lvb_stream_t stream);
+LVB_API int lvb_kv8_append_strided(const uint16_t *query, int64_t query_token_stride, uint16_t *query_out,
+                                   int64_t query_out_stride, const uint16_t *key, int64_t key_token_stride,
+                                   const uint16_t *value, int64_t value_token_stride, const int32_t *positions,
+                                   const uint16_t *cos_table, const uint16_t *sin_table, int64_t table_rows,
+                                   void *key_codes, void *value_codes, float *key_scales, float *value_scales,
+                                   const int32_t *block_tables, int64_t table_cols, int64_t table_stride,
+                                   const int32_t *num_computed, const int32_t *query_start_loc, int64_t num_seqs,
+                                   int64_t num_tokens, int64_t max_query_len, int64_t num_query_heads,
+                                   int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks,
+                                   int dtype, int code_type, lvb_stream_t stream);
 
 /* Values of whole blocks: key_out / value_out [num_ids][num_kv_heads]
  * [block_size][head_size] of `dtype`, code * scale rounded once; zeros for a
@@ -563,7 +575,9 @@ LVB_API int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, 
  * (the longest context) bounds nothing and need not be exact.  workspace: the bytes
  * that lvb_kv8_attention_workspace_bytes gives for the same arguments (0:
  * none), 16-byte aligned, zero-filled once; every call leaves it as it needs
- * it.  Calls sharing a workspace must not overlap on the GPU. */
+ * it.  Calls sharing a workspace must not overlap on the GPU.  The table has
+ * table_stride columns; lvb_kv8_attention_strided takes the columns and the
+ * row stride apart. */
 LVB_API size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
                                                  int64_t head_size, int64_t max_query_len, int64_t max_seq_len);
 LVB_API int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
@@ -574,6 +588,15 @@ LVB_API int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride,
                               int64_t num_query_heads, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
                               int64_t num_blocks, float scale, int dtype, int code_type, void *workspace,
                               size_t workspace_bytes, lvb_stream_t stream);
+LVB_API int lvb_kv8_attention_strided(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
+                                      const void *value_codes, const float *key_scales, const float *value_scales,
+                                      uint16_t *out, int64_t out_token_stride, const int32_t *block_tables,
+                                      int64_t table_cols, int64_t table_stride, const int32_t *num_computed,
+                                      const int32_t *query_start_loc, int64_t num_seqs, int64_t num_tokens,
+                                      int64_t max_query_len, int64_t max_seq_len, int64_t num_query_heads,
+                                      int64_t num_kv_heads, int64_t head_size, int64_t block_size,
+                                      int64_t num_blocks, float scale, int dtype, int code_type, void *workspace,
+                                      size_t workspace_bytes, lvb_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Verification of drafted tokens                                            */

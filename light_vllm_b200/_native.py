@@ -20,7 +20,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblvb200.so"
 HOSTPACK_PATH = Path(__file__).resolve().parent / "_lib" / ("_hostpack" + sysconfig.get_config_var("EXT_SUFFIX"))
 TORCH_OPS_PATH = HOSTPACK_PATH.with_name("_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 LVB_OK = 0
 LVB_ERR_INVALID = 1
@@ -142,6 +142,11 @@ PROTOTYPES: dict[str, tuple[object, tuple[object, ...]]] = {
         (_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr,
          _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _c_ptr),
     ),
+    "lvb_kv8_append_strided": (
+        _int,
+        (_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr,
+         _c_ptr, _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _c_ptr),
+    ),
     "lvb_kv8_read_blocks": (
         _int,
         (_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _int, _int, _c_ptr),
@@ -150,6 +155,11 @@ PROTOTYPES: dict[str, tuple[object, tuple[object, ...]]] = {
     "lvb_kv8_attention": (
         _int,
         (_c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _c_ptr, _size, _c_ptr),
+    ),
+    "lvb_kv8_attention_strided": (
+        _int,
+        (_c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64,
          _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _c_ptr, _size, _c_ptr),
     ),
     "lvb_verify_drafts_workspace_bytes": (_size, (_i64, _i64)),
@@ -238,7 +248,7 @@ def torch_ops():
     loader.exec_module(module)
     lib = library()
     module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                  for name in ("lvb_kv8_append", "lvb_kv8_read_blocks", "lvb_kv8_attention",
+                  for name in ("lvb_kv8_append_strided", "lvb_kv8_read_blocks", "lvb_kv8_attention_strided",
                                "lvb_kv8_attention_workspace_bytes", "lvb_verify_drafts",
                                "lvb_verify_drafts_workspace_bytes")))
     return module

@@ -84,6 +84,7 @@ struct Pair<true> {
 struct Step {
   const int32_t *tables;
   int64_t table_stride;
+  int table_cols;  // blocks of a row; the stride may be anything (a slice of a wider buffer, one row for all requests)
   const int32_t *computed;
   const int32_t *qsl;
   int num_seqs, num_tokens, max_query_len;
@@ -99,7 +100,7 @@ __device__ __forceinline__ bool request_range(const Step &s, int r, int &q0, int
   computed = s.computed[r];
   qlen = q1 - q0;
   if (q0 < 0 || qlen < 0 || q1 > s.num_tokens || computed < 0 || qlen > s.max_query_len ||
-      static_cast<int64_t>(computed) + qlen > s.table_stride * s.bs) {
+      static_cast<int64_t>(computed) + qlen > static_cast<int64_t>(s.table_cols) * s.bs) {
     record_device_error(LVB_DEVERR_INDEX);
     return false;
   }

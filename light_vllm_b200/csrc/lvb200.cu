@@ -37,7 +37,7 @@
 
 namespace {
 
-constexpr int kAbiVersion = 9;
+constexpr int kAbiVersion = 10;
 constexpr int kMaxDevices = 64;
 
 thread_local char g_last_error[512] = "";
@@ -2088,13 +2088,14 @@ int lvb_silu_mul(const uint16_t *gate_up, int64_t in_stride, int64_t tokens, int
 namespace {
 
 // Checks shared by the entry points over the 8-bit cache; fills `s`.
-int kv8_step(const char *what, lvb::kv8::Step &s, const int32_t *tables, int64_t table_stride, const int32_t *computed,
-             const int32_t *qsl, int64_t num_seqs, int64_t num_tokens, int64_t max_query_len, int64_t hkv, int64_t d,
+int kv8_step(const char *what, lvb::kv8::Step &s, const int32_t *tables, int64_t table_cols, int64_t table_stride,
+             const int32_t *computed, const int32_t *qsl, int64_t num_seqs, int64_t num_tokens, int64_t max_query_len, int64_t hkv, int64_t d,
              int64_t bs, int64_t num_blocks, int dtype, int code) {
   if (dtype != LVB_DTYPE_F16 && dtype != LVB_DTYPE_BF16) return fail(LVB_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
   if (code != LVB_KV8_INT8 && code != LVB_KV8_E4M3) return fail(LVB_ERR_INVALID, "%s: unknown code type %d", what, code);
   if (num_seqs < 0 || num_seqs > 65535 || num_tokens < 0 || num_tokens > INT_MAX || max_query_len < 0 ||
-      max_query_len > INT_MAX || table_stride < 0 || table_stride > INT_MAX || num_blocks <= 0 || num_blocks > INT_MAX)
+      max_query_len > INT_MAX || table_cols < 0 || table_cols > INT_MAX || table_stride < 0 || table_stride > INT_MAX ||
+      num_blocks <= 0 || num_blocks > INT_MAX)
     return fail(LVB_ERR_INVALID, "%s: invalid batch size", what);
   if (hkv <= 0 || hkv > 65535) return fail(LVB_ERR_INVALID, "%s: invalid KV head count %lld", what, (long long)hkv);
   if (d != 64 && d != 128)
@@ -2106,6 +2107,7 @@ int kv8_step(const char *what, lvb::kv8::Step &s, const int32_t *tables, int64_t
   if (num_seqs > 0 && (!tables || !computed || !qsl)) return fail(LVB_ERR_INVALID, "%s: null pointer argument", what);
   s.tables = tables;
   s.table_stride = table_stride;
+  s.table_cols = static_cast<int>(table_cols);
   s.computed = computed;
   s.qsl = qsl;
   s.num_seqs = static_cast<int>(num_seqs);
@@ -2145,8 +2147,24 @@ int lvb_kv8_append(const uint16_t *query, int64_t query_token_stride, uint16_t *
                    const int32_t *query_start_loc, int64_t num_seqs, int64_t num_tokens, int64_t max_query_len,
                    int64_t num_query_heads, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
                    int64_t num_blocks, int dtype, int code_type, lvb_stream_t stream) {
+  return lvb_kv8_append_strided(query, query_token_stride, query_out, query_out_stride, key, key_token_stride, value,
+                                value_token_stride, positions, cos_table, sin_table, table_rows, key_codes, value_codes,
+                                key_scales, value_scales, block_tables, table_stride, table_stride, num_computed,
+                                query_start_loc, num_seqs, num_tokens, max_query_len, num_query_heads, num_kv_heads,
+                                head_size, block_size, num_blocks, dtype, code_type, stream);
+}
+
+int lvb_kv8_append_strided(const uint16_t *query, int64_t query_token_stride, uint16_t *query_out,
+                           int64_t query_out_stride, const uint16_t *key, int64_t key_token_stride,
+                           const uint16_t *value, int64_t value_token_stride, const int32_t *positions,
+                           const uint16_t *cos_table, const uint16_t *sin_table, int64_t table_rows, void *key_codes,
+                           void *value_codes, float *key_scales, float *value_scales, const int32_t *block_tables,
+                           int64_t table_cols, int64_t table_stride, const int32_t *num_computed,
+                           const int32_t *query_start_loc, int64_t num_seqs, int64_t num_tokens, int64_t max_query_len,
+                           int64_t num_query_heads, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
+                           int64_t num_blocks, int dtype, int code_type, lvb_stream_t stream) {
   lvb::kv8::AppendArgs a{};
-  int rc = kv8_step("kv8_append", a.step, block_tables, table_stride, num_computed, query_start_loc, num_seqs,
+  int rc = kv8_step("kv8_append", a.step, block_tables, table_cols, table_stride, num_computed, query_start_loc, num_seqs,
                     num_tokens, max_query_len, num_kv_heads, head_size, block_size, num_blocks, dtype, code_type);
   if (rc != LVB_OK) return rc;
   if (num_query_heads < 0 || num_query_heads > 65535 || num_query_heads * num_tokens > INT_MAX)
@@ -2202,7 +2220,7 @@ int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, const fl
                         uint16_t *value_out, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
                         int64_t num_blocks, int dtype, int code_type, lvb_stream_t stream) {
   lvb::kv8::Step s{};
-  int rc = kv8_step("kv8_read_blocks", s, nullptr, 0, nullptr, nullptr, 0, 0, 0, num_kv_heads, head_size, block_size,
+  int rc = kv8_step("kv8_read_blocks", s, nullptr, 0, 0, nullptr, nullptr, 0, 0, 0, num_kv_heads, head_size, block_size,
                     num_blocks, dtype, code_type);
   if (rc != LVB_OK) return rc;
   if (num_ids < 0 || num_ids > INT_MAX) return fail(LVB_ERR_INVALID, "kv8_read_blocks: invalid block count");
@@ -2320,8 +2338,24 @@ int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const v
                       int64_t num_tokens, int64_t max_query_len, int64_t max_seq_len, int64_t num_query_heads,
                       int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks, float scale,
                       int dtype, int code_type, void *workspace, size_t workspace_bytes, lvb_stream_t stream) {
+  return lvb_kv8_attention_strided(query, query_token_stride, key_codes, value_codes, key_scales, value_scales, out,
+                                   out_token_stride, block_tables, table_stride, table_stride, num_computed,
+                                   query_start_loc, num_seqs, num_tokens, max_query_len, max_seq_len, num_query_heads,
+                                   num_kv_heads, head_size, block_size, num_blocks, scale, dtype, code_type, workspace,
+                                   workspace_bytes, stream);
+}
+
+int lvb_kv8_attention_strided(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
+                              const void *value_codes, const float *key_scales, const float *value_scales,
+                              uint16_t *out, int64_t out_token_stride, const int32_t *block_tables,
+                              int64_t table_cols, int64_t table_stride, const int32_t *num_computed,
+                              const int32_t *query_start_loc, int64_t num_seqs, int64_t num_tokens,
+                              int64_t max_query_len, int64_t max_seq_len, int64_t num_query_heads,
+                              int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks,
+                              float scale, int dtype, int code_type, void *workspace, size_t workspace_bytes,
+                              lvb_stream_t stream) {
   lvb::kv8::AttnArgs a{};
-  int rc = kv8_step("kv8_attention", a.step, block_tables, table_stride, num_computed, query_start_loc, num_seqs,
+  int rc = kv8_step("kv8_attention", a.step, block_tables, table_cols, table_stride, num_computed, query_start_loc, num_seqs,
                     num_tokens, max_query_len, num_kv_heads, head_size, block_size, num_blocks, dtype, code_type);
   if (rc != LVB_OK) return rc;
   if (num_query_heads <= 0 || num_query_heads % num_kv_heads || num_query_heads > 65535)

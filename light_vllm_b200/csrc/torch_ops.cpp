@@ -29,9 +29,9 @@
 
 namespace {
 
-decltype(&lvb_kv8_append) g_append;
+decltype(&lvb_kv8_append_strided) g_append;
 decltype(&lvb_kv8_read_blocks) g_read;
-decltype(&lvb_kv8_attention) g_attention;
+decltype(&lvb_kv8_attention_strided) g_attention;
 decltype(&lvb_kv8_attention_workspace_bytes) g_attention_bytes;
 decltype(&lvb_verify_drafts) g_verify;
 decltype(&lvb_verify_drafts_workspace_bytes) g_verify_bytes;
@@ -182,7 +182,7 @@ PyObject *attention(PyObject *const *args) {
   const at::Tensor out = given ? *given : fresh({tokens, hq, l.d}, q->scalar_type());
   const int status = g_attention(
       data<uint16_t>(*q), q->stride(0), data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]),
-      data<float>(*l.t[3]), data<uint16_t>(out), out.stride(0), data<int32_t>(*s.tables), s.tables->stride(0),
+      data<float>(*l.t[3]), data<uint16_t>(out), out.stride(0), data<int32_t>(*s.tables), s.tables->size(1), s.tables->stride(0),
       data<int32_t>(*s.computed), data<int32_t>(*s.start), s.n, tokens, s.max_query, s.max_seq, hq, l.hkv, l.d, l.bs,
       l.blocks, static_cast<float>(scale), act, l.code, ws.ptr, ws.bytes, handle(stream));
   if (status == LVB_OK && given) {
@@ -233,7 +233,7 @@ PyObject *append(PyObject *const *args) {
       query ? out.stride(0) : 0, data<uint16_t>(*key), key->stride(0), data<uint16_t>(*value), value->stride(0),
       pos ? data<int32_t>(*pos) : nullptr, cos ? data<uint16_t>(*cos) : nullptr, sin ? data<uint16_t>(*sin) : nullptr,
       cos ? cos->size(0) : 0, data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]), data<float>(*l.t[3]),
-      data<int32_t>(*s.tables), s.tables->stride(0), data<int32_t>(*s.computed), data<int32_t>(*s.start), s.n, tokens,
+      data<int32_t>(*s.tables), s.tables->size(1), s.tables->stride(0), data<int32_t>(*s.computed), data<int32_t>(*s.start), s.n, tokens,
       s.max_query, hq, l.hkv, l.d, l.bs, l.blocks, act, l.code, handle(stream));
   if (status != LVB_OK) return PyLong_FromLong(status);
   if (given) {

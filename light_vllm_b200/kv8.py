@@ -61,7 +61,7 @@ class KV8Step(NamedTuple):
     longest context (computed and query tokens); results do not depend on the
     latter."""
 
-    block_tables: Tensor  # [requests, blocks]
+    block_tables: Tensor  # [requests, blocks], rows at any stride
     num_computed: Tensor  # [requests], tokens cached by earlier steps
     query_start: Tensor  # [requests + 1], prefix sums of query lengths
     max_query_len: int
@@ -222,11 +222,11 @@ def kv8_append(query: Tensor | None, key: Tensor, value: Tensor, layer: KV8Layer
                                                 query_out.stride(0))
     if tokens and n:
         with _on(index):
-            _native.check(_native.library().lvb_kv8_append(
+            _native.check(_native.library().lvb_kv8_append_strided(
                 q_ptr, q_stride, out_ptr, out_stride, key.data_ptr(), key.stride(0), value.data_ptr(),
                 value.stride(0), pos_ptr, cos_ptr, sin_ptr, table_rows, keys.data_ptr(), layer.values.data_ptr(),
                 layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), step.block_tables.data_ptr(),
-                step.block_tables.stride(0), step.num_computed.data_ptr(), step.query_start.data_ptr(), n, tokens,
+                step.block_tables.shape[1], step.block_tables.stride(0), step.num_computed.data_ptr(), step.query_start.data_ptr(), n, tokens,
                 step.max_query_len, hq, hkv, d, block, num_blocks, act, code, _native.stream_handle(device)),
                 "lvb_kv8_append")
     return query_out
@@ -305,11 +305,11 @@ def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float
             stream = _native.stream_handle(device)
             need = lib.lvb_kv8_attention_workspace_bytes(n, hq, hkv, d, step.max_query_len, step.max_seq_len)
             ws, ws_bytes = _workspaces.get(device, stream, need)
-            _native.check(lib.lvb_kv8_attention(
+            _native.check(lib.lvb_kv8_attention_strided(
                 query.data_ptr(), query.stride(0), keys.data_ptr(), layer.values.data_ptr(),
                 layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), out.data_ptr(), out.stride(0),
-                step.block_tables.data_ptr(), step.block_tables.stride(0), step.num_computed.data_ptr(),
-                step.query_start.data_ptr(), n, tokens, step.max_query_len, step.max_seq_len, hq, hkv, d, block,
+                step.block_tables.data_ptr(), step.block_tables.shape[1], step.block_tables.stride(0),
+                step.num_computed.data_ptr(), step.query_start.data_ptr(), n, tokens, step.max_query_len, step.max_seq_len, hq, hkv, d, block,
                 num_blocks, scale, act, code, ws, ws_bytes, stream), "lvb_kv8_attention")
     return out
 
