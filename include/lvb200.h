@@ -502,6 +502,10 @@ LVB_API int lvb_embedding(const int64_t *ids, int64_t tokens, const uint16_t *ta
                           int64_t vocab_end, int64_t hidden_size, uint16_t *out, int64_t out_stride,
                           lvb_stream_t stream);
 
+/* The capture that `stream` is part of, unique in the process; 0: it is not
+ * being captured. */
+LVB_API uint64_t lvb_stream_capture_id(lvb_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* 8-bit paged K/V cache                                                     */
 /* ------------------------------------------------------------------------ */
@@ -574,10 +578,13 @@ LVB_API int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, 
  * of the batch (LVB_DEVERR_INDEX and no output for a longer one); max_seq_len
  * (the longest context) bounds nothing and need not be exact.  workspace: the bytes
  * that lvb_kv8_attention_workspace_bytes gives for the same arguments (0:
- * none), 16-byte aligned, zero-filled once; every call leaves it as it needs
- * it.  Calls sharing a workspace must not overlap on the GPU.  The table has
+ * none), 16-byte aligned, its first LVB_KV8_COUNTER_BYTES zero-filled once;
+ * every call leaves it as it needs it.  Calls sharing a workspace must not
+ * overlap on the GPU, replays of a graph that holds such calls among them (give
+ * every graph a workspace of its own: lvb_stream_capture_id).  The table has
  * table_stride columns; lvb_kv8_attention_strided takes the columns and the
  * row stride apart. */
+#define LVB_KV8_COUNTER_BYTES 16384
 LVB_API size_t lvb_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_query_heads, int64_t num_kv_heads,
                                                  int64_t head_size, int64_t max_query_len, int64_t max_seq_len);
 LVB_API int lvb_kv8_attention(const uint16_t *query, int64_t query_token_stride, const void *key_codes,
@@ -619,7 +626,8 @@ LVB_API int lvb_kv8_attention_strided(const uint16_t *query, int64_t query_token
  * LVB_DEVERR_INDEX.  Weights that are NaN or negative count as 0.  Up to 2^22
  * words (LVB_ERR_UNSUPPORTED above).
  * workspace: lvb_verify_drafts_workspace_bytes() bytes (0: none), 16-byte
- * aligned, zero-filled once; calls sharing one must not overlap on the GPU.
+ * aligned, zero-filled once; calls sharing one must not overlap on the GPU,
+ * replays of a graph among them.
  * The reference accepts drafts by greedy comparison only
  * (runtime/execution/speculative.py). */
 LVB_API size_t lvb_verify_drafts_workspace_bytes(int64_t num_seqs, int64_t vocab_size);

@@ -20,7 +20,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblvb200.so"
 HOSTPACK_PATH = Path(__file__).resolve().parent / "_lib" / ("_hostpack" + sysconfig.get_config_var("EXT_SUFFIX"))
 TORCH_OPS_PATH = HOSTPACK_PATH.with_name("_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 LVB_OK = 0
 LVB_ERR_INVALID = 1
@@ -34,6 +34,7 @@ DTYPE_BF16 = 1
 
 KV8_INT8 = 0
 KV8_E4M3 = 1
+KV8_COUNTER_BYTES = 16384
 
 _c_ptr = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -137,6 +138,7 @@ PROTOTYPES: dict[str, tuple[object, tuple[object, ...]]] = {
          _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int,
          _c_ptr, _size, _c_ptr),
     ),
+    "lvb_stream_capture_id": (ctypes.c_uint64, (_c_ptr,)),
     "lvb_kv8_append": (
         _int,
         (_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr, _i64, _c_ptr, _c_ptr, _c_ptr,
@@ -210,6 +212,12 @@ def stream_handle(device) -> int:
     return _raw_stream(index)
 
 
+def stream_capture_id(stream: int) -> int:
+    """The capture that ``stream`` (a raw handle) is part of; 0: none."""
+
+    return library().lvb_stream_capture_id(stream)
+
+
 def _raw_stream(index: int) -> int:
     import torch
 
@@ -250,7 +258,7 @@ def torch_ops():
     module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                   for name in ("lvb_kv8_append_strided", "lvb_kv8_read_blocks", "lvb_kv8_attention_strided",
                                "lvb_kv8_attention_workspace_bytes", "lvb_verify_drafts",
-                               "lvb_verify_drafts_workspace_bytes")))
+                               "lvb_verify_drafts_workspace_bytes", "lvb_stream_capture_id")))
     return module
 
 

@@ -37,7 +37,7 @@
 
 namespace {
 
-constexpr int kAbiVersion = 10;
+constexpr int kAbiVersion = 11;
 constexpr int kMaxDevices = 64;
 
 thread_local char g_last_error[512] = "";
@@ -2082,6 +2082,16 @@ int lvb_silu_mul(const uint16_t *gate_up, int64_t in_stride, int64_t tokens, int
   return e == cudaSuccess ? LVB_OK : cuda_fail(e, "silu_mul_kernel launch");
 }
 
+uint64_t lvb_stream_capture_id(lvb_stream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // (the legacy stream beside another's capture)
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 // ------------------------------------------------------------------------
 // 8-bit paged cache and draft verification
 // ------------------------------------------------------------------------
@@ -2253,8 +2263,8 @@ int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, const fl
 
 namespace {
 
-// Workspace of an attention call: the CTAs' counters first, at the same place
-// for every call on a device, so that they stay zero whatever calls share a
+// Workspace of an attention call: the CTAs' counters first (20 bytes an SM), at
+// the same place for every call, so that they stay zero whatever calls share a
 // buffer; then two pieces for each CTA of the decode kernel, and, where a
 // request may have more rows than that takes, of the tile kernel.
 struct Kv8Workspace {
@@ -2286,7 +2296,7 @@ Kv8Workspace kv8_workspace(int sms, bool tiles) {
   const size_t rows = static_cast<size_t>(2) * sms * lvb::kv8::kMaxRows<64>, tile_rows = tiles ? static_cast<size_t>(2) * sms * lvb::kv8::kTileRows : 0;
   Kv8Workspace w{};
   w.tile_counts = round256(static_cast<size_t>(sms) * kKv8DecodeCtasPerSm * 4);
-  w.o = w.tile_counts + round256(static_cast<size_t>(sms) * 4);
+  w.o = std::max<size_t>(LVB_KV8_COUNTER_BYTES, w.tile_counts + round256(static_cast<size_t>(sms) * 4));
   w.ml = w.o + rows * 128 * sizeof(float);
   w.tile_o = round256(w.ml + rows * sizeof(float2));
   w.tile_ml = w.tile_o + tile_rows * 128 * sizeof(float);

@@ -7,7 +7,8 @@
 // (the types, shapes, strides and devices that need no copy), allocates the
 // outputs through torch, finds the workspace of the current stream and calls the
 // C entry point.  Anything else -- a malformed argument, rows that need a copy,
-// another device than the current one, a workspace that does not exist yet --
+// another device than the current one, a workspace that does not exist yet, a
+// stream under capture (its graph's workspace is its own) --
 // returns None with nothing done, and the Python wrapper (kv8.py,
 // speculative.py), which knows every rule and message, takes the call.  A status
 // other than 0 of the entry point is returned as an int.
@@ -35,6 +36,7 @@ decltype(&lvb_kv8_attention_strided) g_attention;
 decltype(&lvb_kv8_attention_workspace_bytes) g_attention_bytes;
 decltype(&lvb_verify_drafts) g_verify;
 decltype(&lvb_verify_drafts_workspace_bytes) g_verify_bytes;
+decltype(&lvb_stream_capture_id) g_capture;
 
 // Scratch of each (operator, device, stream), given by the Python side, which keeps it alive.
 struct Scratch {
@@ -47,6 +49,7 @@ enum { kAttentionScratch = 0, kVerifyScratch = 1 };
 bool scratch(int op, int device, cudaStream_t stream, size_t need, Scratch &out) {
   out = {nullptr, 0};
   if (need == 0) return true;
+  if (g_capture(reinterpret_cast<lvb_stream_t>(stream)) != 0) return false;
   const auto it = g_scratch.find({op, {device, reinterpret_cast<uintptr_t>(stream)}});
   if (it == g_scratch.end() || it->second.bytes < need) return false;
   out = it->second;
@@ -312,16 +315,17 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
 }
 
-// bind(append, read_blocks, attention, attention_bytes, verify, verify_bytes): library entry points
+// bind(append, read_blocks, attention, attention_bytes, verify, verify_bytes, capture): library entry points
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long p[6];
-  if (!PyArg_ParseTuple(args, "KKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5)) return nullptr;
+  unsigned long long p[7];
+  if (!PyArg_ParseTuple(args, "KKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6)) return nullptr;
   g_append = reinterpret_cast<decltype(g_append)>(p[0]);
   g_read = reinterpret_cast<decltype(g_read)>(p[1]);
   g_attention = reinterpret_cast<decltype(g_attention)>(p[2]);
   g_attention_bytes = reinterpret_cast<decltype(g_attention_bytes)>(p[3]);
   g_verify = reinterpret_cast<decltype(g_verify)>(p[4]);
   g_verify_bytes = reinterpret_cast<decltype(g_verify_bytes)>(p[5]);
+  g_capture = reinterpret_cast<decltype(g_capture)>(p[6]);
   Py_RETURN_NONE;
 }
 

@@ -125,33 +125,40 @@ def _dense_heads(rows: Tensor) -> Tensor:
 
 
 class _Workspaces:
-    """Zero-filled scratch of one operator for each (device, stream); a call leaves it as it
-    needs it, and calls on one stream follow one another.  A grown buffer keeps
-    its predecessors, which a captured graph may still name."""
+    """Scratch of one operator, zero where its calls want it and left so by them: a
+    buffer for each (device, stream), whose calls follow one another, and for
+    each capture a buffer of its own in the graph's memory, zeroed by the graph,
+    since a graph may be replayed on any stream, beside whatever runs there."""
 
-    def __init__(self, op: int) -> None:
+    def __init__(self, op: int, zero_bytes: int | None = None) -> None:
         self._op = op
+        self._zero_bytes = zero_bytes  # that have to be zero (None: all of it)
         self._current: dict[tuple[int, int], Tensor] = {}
-        self._kept: list[Tensor] = []
+        self._captured: dict[tuple[int, int], tuple[int, Tensor]] = {}
 
     def get(self, device: torch.device, stream: int, need: int) -> tuple[int, int]:
         if need == 0:
             return 0, 0
         key = (device.index, stream)
+        capture = _native.stream_capture_id(stream)
+        if capture:
+            held, buf = self._captured.get(key, (0, None))
+            if held != capture or buf.numel() < need:
+                buf = torch.empty(need, dtype=torch.uint8, device=device)
+                buf[:self._zero_bytes].zero_()
+                # (former captures' buffers go back to their graphs' memory)
+                self._captured = {k: v for k, v in self._captured.items() if v[0] == capture}
+                self._captured[key] = capture, buf
+            return buf.data_ptr(), buf.numel()
         buf = self._current.get(key)
         if buf is None or buf.numel() < need:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("run the operator once on this stream before capturing it: its workspace is not "
-                                   "allocated yet")
-            if buf is not None:
-                self._kept.append(buf)
             buf = torch.zeros(max(1 << 20, 1 << (need - 1).bit_length()), dtype=torch.uint8, device=device)
             self._current[key] = buf
             _native.torch_ops().set_scratch(self._op, device.index, stream, buf.data_ptr(), buf.numel())
         return buf.data_ptr(), buf.numel()
 
 
-_workspaces = _Workspaces(0)
+_workspaces = _Workspaces(0, _native.KV8_COUNTER_BYTES)
 _fast = None  # _torch_ops, loaded by the first call
 
 
