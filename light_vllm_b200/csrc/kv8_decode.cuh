@@ -10,7 +10,9 @@
 //     O = sum_j 2^(x_j - m) value code_j        L = sum_j 2^(x_j - m) / w_b
 // give out = O / L: the value scale rides in the exponent, so the weights that
 // enter the second product lie in (0, 1] whatever the scales are, and no code is
-// ever multiplied by a scale.  They enter it as fp16, times 2^6 (kHead) and up to
+// ever multiplied by a scale.  (w_b = 0, a block of zeros, stands as kZeroWeight,
+// below every live block's: it adds to L and does not raise m, which would push the
+// others' weights out of fp16.)  They enter it as fp16, times 2^6 (kHead) and up to
 // 2^8 (kLazy) more, so that a weight 2^-20 of the largest still has 11 bits; O, L,
 // m and the scores are fp32.  m moves only when it would grow by more than kLazy:
 // a rescaling of O is rare.
@@ -52,6 +54,9 @@ namespace kv8 {
 
 constexpr float kHead = 6.f;
 constexpr float kLazy = 8.f;
+// With it L stays below 2^(80 + 6 + 8) for each position, and a weight at the least
+// scale that append keeps, 2^-100, is a normal fp16 beside a block of zeros.
+constexpr float kZeroWeight = 0x1p-80f;
 constexpr int kPage = 16;     // positions a warp takes at a time
 // Query rows of a decode item (their O in registers: 80 of them at 40 x 64).
 template <int D>
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, kNT>::kThreads, DecodeCfg<D, kNT>
       float y[kPages][kNT][4], lw[kPages], iw[kPages];
 #pragma unroll
       for (int i = 0; i < kPages; ++i) {
-        const float vw = (now >> i & 1u) && vs[i] > 0.f ? vs[i] : 1.f;  // (a page that does not exist brings no scales)
+        const float vw = (now >> i & 1u) && vs[i] > 0.f ? vs[i] : kZeroWeight;  // (a page that does not exist brings no scales)
         lw[i] = log2_fast(vw);
         iw[i] = rcp_fast(vw);
       }

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __g
       if (have) {
         if (warp == 8) {
           if (lane < 8) {
-            const float kw = ksc > 0.f ? ksc : 1.f, vw = vsc > 0.f ? vsc : 1.f;  // (scale 0: codes 0)
+            const float kw = ksc > 0.f ? ksc : 1.f, vw = vsc > 0.f ? vsc : kZeroWeight;  // (key scale 0: codes 0)
             // a page that does not exist weighs nothing
             scale_sm[(g & 3) * 8 + lane] =
                 ksc < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f) : make_float4(kw, log2_fast(vw), rcp_fast(vw), 0.f);
