@@ -220,7 +220,7 @@ template <bool kBf16, bool kFp8, int D>
 __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __grid_constant__ AttnArgs a) {
   using Cfg = TileCfg<D>;
   constexpr float kNone = -1e30f;
-  constexpr float kLeast = 1.2e-38f;  // a factor that leaves -inf what it is
+  constexpr float kLeast = 1.2e-38f;  // a factor that leaves -inf what it is, and makes 0 of every score
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float4 *scale_sm = reinterpret_cast<float4 *>(smem + Cfg::kScaleOff);
@@ -393,10 +393,10 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1) tile_kernel(const __g
       if (have) {
         if (warp == 8) {
           if (lane < 8) {
-            const float kw = ksc > 0.f ? ksc : 1.f, vw = vsc > 0.f ? vsc : kZeroWeight;  // (key scale 0: codes 0)
+            const float vw = vsc > 0.f ? vsc : kZeroWeight;
             // a page that does not exist weighs nothing
             scale_sm[(g & 3) * 8 + lane] =
-                ksc < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f) : make_float4(kw, log2_fast(vw), rcp_fast(vw), 0.f);
+                ksc < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f) : make_float4(ksc, log2_fast(vw), rcp_fast(vw), 0.f);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(sc_full + (g & 3));

@@ -76,12 +76,21 @@ def _as_if_zero(layer, blocks, side):
     return stale, stale._replace(**{side + "s": codes})
 
 
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_codes_under_a_key_scale_of_zero(batch, code):
+    """A code stands for code * scale: under a scale that was set to zero it is a zero, bit for bit."""
+
+    query, layer, step, tables, requests = _case(batch, (14, 2, 64), code, 3)
+    stale, zeros = _as_if_zero(layer, sum((t[::2] for t in tables), []), "key")
+    assert torch.equal(kv8_attention(query, stale, step, scale=0.125), kv8_attention(query, zeros, step, scale=0.125))
+    _check(query, stale, step, tables, requests, code, 0.125)
+
+
 @pytest.mark.parametrize("size", [1.0, 2.0 ** -40])
 @pytest.mark.parametrize("batch", BATCHES)
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 def test_codes_under_a_value_scale_of_zero(batch, code, size):
-    """A code stands for code * scale: under a scale that was set to zero it is a zero, bit for bit."""
-
     query, layer, step, tables, _ = _case(batch, (14, 2, 64), code, 4, size)
     stale, zeros = _as_if_zero(layer, sum((t[::2] for t in tables), []), "value")
     assert torch.equal(kv8_attention(query, stale, step, scale=0.125), kv8_attention(query, zeros, step, scale=0.125))
