@@ -127,8 +127,11 @@ bool step(PyObject *const *args, int device, Step &s) {
 bool rows(const at::Tensor *t, int64_t tokens, int64_t heads, int64_t d, at::ScalarType type, int device) {
   if (!t || t->dim() != 3 || t->scalar_type() != type || !t->is_cuda() || t->get_device() != device) return false;
   if (t->size(0) != tokens || (heads >= 0 && t->size(1) != heads) || t->size(2) != d) return false;
-  return t->stride(2) == 1 && (t->size(1) <= 1 || t->stride(1) == d) && t->stride(0) >= t->size(1) * d;
+  return t->stride(2) == 1 && (t->size(1) <= 1 || t->stride(1) == d) && (tokens == 1 || t->stride(0) >= t->size(1) * d);
 }
+
+// Elements from token to token; a single one's stride means nothing.
+int64_t token_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
 
 // A new tensor on the current device, from torch's caching allocator without
 // the dispatcher (about 1 us less than at::empty).
@@ -138,7 +141,7 @@ at::Tensor fresh(at::IntArrayRef size, at::ScalarType type) {
 }
 
 // Whether rows may be read and written 16 bytes at a time.
-bool aligned(const at::Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % 8 == 0; }
+bool aligned(const at::Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && token_stride(t) % 8 == 0; }
 
 int act_of(const at::Tensor &t) {
   return t.scalar_type() == at::kHalf ? LVB_DTYPE_F16 : t.scalar_type() == at::kBFloat16 ? LVB_DTYPE_BF16 : -1;
@@ -184,8 +187,8 @@ PyObject *attention(PyObject *const *args) {
     Py_RETURN_NONE;
   const at::Tensor out = given ? *given : fresh({tokens, hq, l.d}, q->scalar_type());
   const int status = g_attention(
-      data<uint16_t>(*q), q->stride(0), data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]),
-      data<float>(*l.t[3]), data<uint16_t>(out), out.stride(0), data<int32_t>(*s.tables), s.tables->size(1), s.tables->stride(0),
+      data<uint16_t>(*q), token_stride(*q), data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]),
+      data<float>(*l.t[3]), data<uint16_t>(out), token_stride(out), data<int32_t>(*s.tables), s.tables->size(1), s.tables->stride(0),
       data<int32_t>(*s.computed), data<int32_t>(*s.start), s.n, tokens, s.max_query, s.max_seq, hq, l.hkv, l.d, l.bs,
       l.blocks, static_cast<float>(scale), act, l.code, ws.ptr, ws.bytes, handle(stream));
   if (status == LVB_OK && given) {
@@ -232,8 +235,8 @@ PyObject *append(PyObject *const *args) {
   if (query) out = given ? *given : fresh({tokens, hq, l.d}, type);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(l.device)).stream();
   const int status = g_append(
-      query ? data<uint16_t>(*query) : nullptr, query ? query->stride(0) : 0, query ? data<uint16_t>(out) : nullptr,
-      query ? out.stride(0) : 0, data<uint16_t>(*key), key->stride(0), data<uint16_t>(*value), value->stride(0),
+      query ? data<uint16_t>(*query) : nullptr, query ? token_stride(*query) : 0, query ? data<uint16_t>(out) : nullptr,
+      query ? token_stride(out) : 0, data<uint16_t>(*key), token_stride(*key), data<uint16_t>(*value), token_stride(*value),
       pos ? data<int32_t>(*pos) : nullptr, cos ? data<uint16_t>(*cos) : nullptr, sin ? data<uint16_t>(*sin) : nullptr,
       cos ? cos->size(0) : 0, data<void>(*l.t[0]), data<void>(*l.t[1]), data<float>(*l.t[2]), data<float>(*l.t[3]),
       data<int32_t>(*s.tables), s.tables->size(1), s.tables->stride(0), data<int32_t>(*s.computed), data<int32_t>(*s.start), s.n, tokens,

@@ -118,10 +118,18 @@ def _check_rows(name: str, rows: Tensor, tokens: int, heads: int | None, head_si
 def _dense_heads(rows: Tensor) -> Tensor:
     """Rows whose heads are dense and in order (a token's stride is free)."""
 
-    if rows.is_contiguous() or (rows.stride(2) == 1 and rows.stride(1) == rows.shape[2]
-                                and rows.stride(0) >= rows.shape[1] * rows.shape[2]):
+    tokens, heads, d = rows.shape
+    if rows.is_contiguous() or (rows.stride(2) == 1 and (heads == 1 or rows.stride(1) == d)
+                                and (tokens == 1 or rows.stride(0) >= heads * d)):
         return rows
     return rows.contiguous()
+
+
+def _token_stride(rows: Tensor) -> int:
+    """Elements from token to token; a single one's stride means nothing (torch
+    keeps whatever its storage had), so it is what the heads take."""
+
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1] * rows.shape[2]
 
 
 class _Workspaces:
@@ -225,13 +233,13 @@ def kv8_append(query: Tensor | None, key: Tensor, value: Tensor, layer: KV8Layer
                 raise KVCacheError("KV8 query output rows must have dense heads")
         query = _dense_heads(query)
         hq = query.shape[1]
-        q_ptr, q_stride, out_ptr, out_stride = (query.data_ptr(), query.stride(0), query_out.data_ptr(),
-                                                query_out.stride(0))
+        q_ptr, q_stride, out_ptr, out_stride = (query.data_ptr(), _token_stride(query), query_out.data_ptr(),
+                                                _token_stride(query_out))
     if tokens and n:
         with _on(index):
             _native.check(_native.library().lvb_kv8_append_strided(
-                q_ptr, q_stride, out_ptr, out_stride, key.data_ptr(), key.stride(0), value.data_ptr(),
-                value.stride(0), pos_ptr, cos_ptr, sin_ptr, table_rows, keys.data_ptr(), layer.values.data_ptr(),
+                q_ptr, q_stride, out_ptr, out_stride, key.data_ptr(), _token_stride(key), value.data_ptr(),
+                _token_stride(value), pos_ptr, cos_ptr, sin_ptr, table_rows, keys.data_ptr(), layer.values.data_ptr(),
                 layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), step.block_tables.data_ptr(),
                 step.block_tables.shape[1], step.block_tables.stride(0), step.num_computed.data_ptr(), step.query_start.data_ptr(), n, tokens,
                 step.max_query_len, hq, hkv, d, block, num_blocks, act, code, _native.stream_handle(device)),
@@ -301,10 +309,10 @@ def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float
         out = torch.empty(query.shape, dtype=dtype, device=device)
     else:
         _check_rows("output", out, tokens, hq, d, dtype, index)
-        if _dense_heads(out) is not out or out.data_ptr() % 16 or (tokens > 1 and out.stride(0) % 8):
+        if _dense_heads(out) is not out or out.data_ptr() % 16 or _token_stride(out) % 8:
             raise KVCacheError("KV8 output rows must have dense heads and be 16-byte aligned")
     query = _dense_heads(query)
-    if query.data_ptr() % 16 or query.stride(0) % 8:
+    if query.data_ptr() % 16 or _token_stride(query) % 8:
         query = query.clone(memory_format=torch.contiguous_format)
     if tokens and n:
         with _on(index):
@@ -313,8 +321,8 @@ def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float
             need = lib.lvb_kv8_attention_workspace_bytes(n, hq, hkv, d, step.max_query_len, step.max_seq_len)
             ws, ws_bytes = _workspaces.get(device, stream, need)
             _native.check(lib.lvb_kv8_attention_strided(
-                query.data_ptr(), query.stride(0), keys.data_ptr(), layer.values.data_ptr(),
-                layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), out.data_ptr(), out.stride(0),
+                query.data_ptr(), _token_stride(query), keys.data_ptr(), layer.values.data_ptr(),
+                layer.key_scales.data_ptr(), layer.value_scales.data_ptr(), out.data_ptr(), _token_stride(out),
                 step.block_tables.data_ptr(), step.block_tables.shape[1], step.block_tables.stride(0),
                 step.num_computed.data_ptr(), step.query_start.data_ptr(), n, tokens, step.max_query_len, step.max_seq_len, hq, hkv, d, block,
                 num_blocks, scale, act, code, ws, ws_bytes, stream), "lvb_kv8_attention")
