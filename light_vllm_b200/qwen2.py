@@ -45,6 +45,7 @@ from light_vllm_b200 import _native
 from light_vllm_b200.awq import B200AWQScheme
 from light_vllm_b200.collectives import (
     PeerWorkspace,
+    TensorParallelCollectives,
     all_reduce_add_rms_norm,
     awq_column_shard,
     awq_row_shard,
@@ -294,15 +295,14 @@ class Qwen2AWQRunner:
 
     def logits(self, input_ids: Tensor, positions: Tensor, attention, logit_rows: Tensor | None = None) -> Tensor:
         """The step of ``forward``, returning the fp16 logits [rows, vocabulary]
-        (gathered over the vocabulary shards under tensor parallelism): what
-        sampling and the verification of drafts start from."""
+        (gathered over the vocabulary shards under tensor parallelism, which
+        may differ by a row): what sampling and the verification of drafts
+        start from."""
 
         local = torch.mm(self._hidden(input_ids, positions, attention, logit_rows), self.lm_head.t())
         if self.world == 1:
             return local
-        shards = torch.empty((self.world,) + tuple(local.shape), dtype=local.dtype, device=self.device)
-        dist.all_gather_into_tensor(shards, local, group=self.group)
-        return shards.transpose(0, 1).reshape(local.shape[0], -1)
+        return TensorParallelCollectives(self.group).all_gather_last_dim(local, self.layout.vocab_part.sizes)
 
     def _hidden(self, input_ids: Tensor, positions: Tensor, attention, logit_rows: Tensor | None) -> Tensor:
         """The decoder stack: final hidden rows of ``logit_rows`` (every row when None)."""
