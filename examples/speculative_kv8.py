@@ -60,6 +60,9 @@ def generate(runner: Qwen2AWQRunner, cache: KV8Cache, prompts: list[list[int]], 
     accepted drafts.  A prompt's step must fit ``runner.max_tokens``."""
 
     device = runner.device
+    longest = max(map(len, prompts), default=0) + new_tokens
+    if longest - 1 > runner.shape.max_position_embeddings:  # (the last token is not run)
+        raise ValueError(f"the model has {runner.shape.max_position_embeddings} positions, {longest - 1} are needed")
     backend = B200KV8AttentionBackend()
     uniform = torch.Generator(device=device).manual_seed(seed)
     block = cache.config.block_size
@@ -109,6 +112,18 @@ def generate(runner: Qwen2AWQRunner, cache: KV8Cache, prompts: list[list[int]], 
         stats["steps"] += 1
 
 
+def demo_prompts(requests: int) -> list[list[int]]:
+    """Prompts of 16, 21, .. tokens."""
+
+    return [[(r * 31 + j * j) % 512 for j in range(16 + 5 * r)] for r in range(requests)]
+
+
+def step_tokens(prompts: list[list[int]], max_drafts: int) -> int:
+    """Tokens of ``generate``'s longest step: all prompts, or every request's last token and drafts."""
+
+    return max(sum(map(len, prompts)), len(prompts) * (max_drafts + 1))
+
+
 def main() -> None:
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--code", choices=sorted(CODES), default="int8")
@@ -123,8 +138,8 @@ def main() -> None:
     weights = random_shard(shape, 0, 1, device)
     # The last token then weighs most in the next one, so that the output repeats itself and drafts are found.
     weights["model.embed_tokens.weight"] *= 500
-    runner = Qwen2AWQRunner(shape, weights, device, max_tokens=256)
-    prompts = [[(r * 31 + j * j) % 512 for j in range(16 + 5 * r)] for r in range(args.requests)]
+    prompts = demo_prompts(args.requests)
+    runner = Qwen2AWQRunner(shape, weights, device, max_tokens=step_tokens(prompts, args.drafts))
     blocks = sum(-(-(len(p) + args.tokens + args.drafts) // 16) for p in prompts)
     try:
         for drafts in (0, args.drafts):
