@@ -95,9 +95,9 @@ def _check_step(step: KV8Step, device: int) -> int:
     """The number of requests; raises ``KVCacheError`` for a malformed step."""
 
     tables, computed, start = step[:3]
-    n = computed.shape[0]
-    if (tables.dtype != torch.int32 or computed.dtype != torch.int32 or start.dtype != torch.int32
-            or len(tables.shape) != 2 or len(computed.shape) != 1 or tables.shape[0] != n or start.shape != (n + 1,)):
+    n = computed.shape[0] if len(computed.shape) == 1 else -1
+    if (n < 0 or tables.dtype != torch.int32 or computed.dtype != torch.int32 or start.dtype != torch.int32
+            or len(tables.shape) != 2 or tables.shape[0] != n or start.shape != (n + 1,)):
         raise KVCacheError("KV8 step metadata must be int32 [n, blocks], [n] and [n + 1]")
     if (tables.get_device() != device or computed.get_device() != device or start.get_device() != device):
         raise KVCacheError("KV8 step metadata must be on the cache's device")
@@ -205,7 +205,7 @@ def kv8_append(query: Tensor | None, key: Tensor, value: Tensor, layer: KV8Layer
     act = _ACT_DTYPES.get(dtype)
     if act is None:
         raise KVCacheError("KV8 rows must be fp16 or bf16")
-    tokens = key.shape[0]
+    tokens = key.shape[0] if key.dim() else 0
     _check_rows("key", key, tokens, hkv, d, dtype, index)
     _check_rows("value", value, tokens, hkv, d, dtype, index)
     key, value = _dense_heads(key), _dense_heads(value)
@@ -300,7 +300,7 @@ def kv8_attention(query: Tensor, layer: KV8Layer, step: KV8Step, *, scale: float
     act = _ACT_DTYPES.get(dtype)
     if act is None:
         raise KVCacheError("KV8 rows must be fp16 or bf16")
-    tokens = query.shape[0]
+    tokens = query.shape[0] if query.dim() else 0
     _check_rows("query", query, tokens, None, d, dtype, index)
     hq = query.shape[1]
     if hq == 0 or hq % hkv:

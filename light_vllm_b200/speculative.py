@@ -57,7 +57,7 @@ def verify_drafts(target_probs: Tensor, draft_tokens: Tensor, accept_uniform: Te
         raise ValueError("the vocabulary must not be empty")
     if query_start.dtype != torch.int32 or query_start.dim() != 1 or query_start.shape[0] == 0:
         raise ValueError("query_start must be an int32 vector of requests + 1 values")
-    n, drafts = query_start.shape[0] - 1, draft_tokens.shape[0]
+    n, drafts = query_start.shape[0] - 1, draft_tokens.numel()
     if draft_tokens.dtype != torch.int64 or accept_uniform.dtype != torch.float32 or sample_uniform.dtype != torch.float32:
         raise ValueError("draft tokens must be int64 and uniform numbers float32")
     if draft_tokens.dim() != 1 or accept_uniform.shape != draft_tokens.shape or sample_uniform.shape != (n,):
