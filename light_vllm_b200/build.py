@@ -110,10 +110,16 @@ def is_stale() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if it is missing or older than its sources."""
+    """Compile the library if it is missing or older than its sources, and the
+    two modules; the torch module last, since the rest does without it."""
 
     build_hostpack(force)
+    build_library(force, verbose)
     build_torch_ops(force)
+    return OUTPUT
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not force and not is_stale():
         return OUTPUT
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
