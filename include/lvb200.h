@@ -574,7 +574,10 @@ LVB_API int lvb_kv8_read_blocks(const void *key_codes, const void *value_codes, 
  * under verification, prompt chunks, any mix), K and V read from the 8-bit
  * cache, which must hold this step's tokens already (lvb_kv8_append).
  * Query and output rows are 16-byte aligned (token strides multiples of 8).
- * Softmax statistics and sums in fp32.  max_query_len is the longest request
+ * Scores, softmax statistics and sums in fp32; the weights, times their block's
+ * value scale, enter the product with V as fp16 (11 bits; below 2^-20 of the
+ * row's largest fewer, down to none at 2^-31), and bf16 queries that with K as fp16 times a power of two (exact
+ * down to 2^-22 of the row's largest element, fewer bits below).  max_query_len is the longest request
  * of the batch (LVB_DEVERR_INDEX and no output for a longer one); max_seq_len
  * (the longest context) bounds nothing and need not be exact.  workspace: the bytes
  * that lvb_kv8_attention_workspace_bytes gives for the same arguments (0:
@@ -623,7 +626,9 @@ LVB_API int lvb_kv8_attention_strided(const uint16_t *query, int64_t query_token
  * num_accepted: drafts accepted.  A request without rows, with rows outside
  * the batch or with more than max_query_len sets LVB_DEVERR_INDEX and gets -1
  * throughout and 0 accepted.  A drafted token outside the vocabulary is refused and sets
- * LVB_DEVERR_INDEX.  Weights that are NaN or negative count as 0.  Up to 2^22
+ * LVB_DEVERR_INDEX.  Weights that are NaN or negative count as 0, and below
+ * 2^-41 they are never drawn; sample_uniform's steps (2^-24 from a usual fp32
+ * generator) bound what the draw can tell apart.  Up to 2^22
  * words (LVB_ERR_UNSUPPORTED above).
  * workspace: lvb_verify_drafts_workspace_bytes() bytes (0: none), 16-byte
  * aligned, zero-filled once; calls sharing one must not overlap on the GPU,

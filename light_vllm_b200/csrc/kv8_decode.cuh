@@ -41,8 +41,10 @@
 // counter for each item) sums them in order, so results do not depend on timing.
 //
 // Measured: 64 requests of 512 to 4096 tokens, 28/4 heads of 128, int8: 49 us (3.1
-// TB/s; 6 TB/s while pages pass, beside 7 us of start and 5 of joins); 5 tokens each
-// for 32 requests of up to 8000, 14/2 heads of 64: 36 us.
+// TB/s): 25 in which pages pass at about 6 TB/s, 7 of start, 5 of joins, some 8 in
+// which SMs have ended (they are active for 78 of 92 thousand cycles: some reach
+// memory more slowly than others), the launch.  5 tokens each for 32 requests of up
+// to 8000, 14/2 heads of 64: 36 us.
 #pragma once
 
 #include <type_traits>
@@ -72,7 +74,7 @@ struct AttnArgs {
   int64_t out_stride;
   const uint8_t *key_codes, *value_codes;
   const float *key_scales, *value_scales;
-  int hq, group;
+  int group;         // query heads of a KV head
   float scale_log2;  // softmax scale * log2(e)
   int few_rows;      // requests of up to this many query rows are the decode kernel's
   // Pieces of items that cross CTAs, and how many of an item's CTAs are done
@@ -180,8 +182,11 @@ struct DecodeCfg {
   static constexpr int kRows = 8 * kNT;
   static constexpr int kPad = D + 4;                // floats of a row of O in shared memory
   static constexpr int kPages = kNT <= (D == 64 ? 3 : 2) ? 2 : 1;  // pages of a step
-  // An item's queries, sums and joining in pages of the CTA's time.  (With 5 tiles
-  // of rows and heads of 64 they take 14K cycles and a page 280.)
+  // An item's queries, sums and joining in pages of the CTA's time: with 5 tiles
+  // of rows and heads of 64 they take 14K cycles and a page 280.  Measured at 2 to 5
+  // tiles and two groups of 3, heads of 64 and 128, batches of 32 and 64 requests:
+  // 20 is 5 to 22 % slower and 10 up to 33 %, 80 within 6 % either way; 8 requests of
+  // up to 3000 tokens take 40 best too (20: up to 18 % slower, 80: up to 9 %).
   static constexpr int kItemCost = kNT == 1 ? 8 : 40;
   static constexpr int kSide = kPage * D;           // K (or V) of a page
   static constexpr int kRingBytes = kWarps * kPages * 2 * kSide;

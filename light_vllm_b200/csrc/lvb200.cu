@@ -2386,7 +2386,6 @@ int lvb_kv8_attention_strided(const uint16_t *query, int64_t query_token_stride,
   a.value_codes = static_cast<const uint8_t *>(value_codes);
   a.key_scales = key_scales;
   a.value_scales = value_scales;
-  a.hq = static_cast<int>(num_query_heads);
   a.group = static_cast<int>(num_query_heads / num_kv_heads);
   if (!aligned16(query) || !aligned16(out) || query_token_stride % 8 || out_token_stride % 8)
     return fail(LVB_ERR_INVALID, "kv8_attention: query and output rows must be 16-byte aligned");

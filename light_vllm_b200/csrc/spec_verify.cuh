@@ -5,8 +5,10 @@
 // which x_i was drawn; without them q_i is 1 at x_i and 0 elsewhere.  Draft i
 // is accepted while u_i q_i(x_i) < p_i(x_i), u_i uniform in [0, 1).  At the
 // first refusal j the next token is drawn from max(p_j - q_j, 0), and after n
-// acceptances from p_n: emitted tokens then follow the target's distribution
-// exactly.
+// acceptances from p_n: emitted tokens then follow the target's distribution, as
+// finely as the uniform numbers allow.  Those are fp32; a generator's are multiples
+// of 2^-24, so acceptance and draw move in steps of 2^-24, and a token with less of
+// the mass is drawn with probability 0 or 2^-24.
 //
 // The draw inverts the distribution function at a given uniform number in
 // whole numbers: W_v = round(2^40 min(w_v, 1)) (0 for w_v <= 0 and NaN; the sum

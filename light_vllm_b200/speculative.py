@@ -3,8 +3,9 @@
 ``verify_drafts`` accepts or refuses a step's drafted tokens against the
 target model's probabilities, and draws the token that follows the accepted
 ones, from uniform numbers that the caller gives (``lvb_verify_drafts``).  The
-emitted tokens follow the target's distribution exactly, whatever drafted
-them.  The reference accepts drafts by greedy comparison only
+emitted tokens follow the target's distribution, whatever drafted them, in the
+steps of the uniform numbers: fp32 ones from a generator are multiples of 2^-24,
+so a token of less probability is drawn with probability 0 or 2^-24.  The reference accepts drafts by greedy comparison only
 (runtime/execution/speculative.py); target probabilities that are 1 at the
 greedy token give that rule.
 """
